@@ -57,6 +57,10 @@ const char *npd_last_error(void);
  * and waits for `stream`.  Returns the word in *out.                                  */
 int npd_read_status(int32_t *status_dev, int32_t *out, void *stream);
 
+/* The id of the capture that `stream` is in, 0 when it is not being captured: for hosts that give
+ * every captured graph scratch of its own.                                             */
+int npd_capture_id(void *stream, uint64_t *id);
+
 /* ---- (1) paged KV store ---------------------------------------------------------
  * Replaces paged_kv_store (nanoPD/paged_attention/csrc/kvstore/paged_kv_store.h:23-27,
  * paged_kv_store_ops.cu:7-50, paged_kv_store_kernel.cu:16-58).
@@ -231,6 +235,49 @@ int64_t npd_top_k_sample_workspace_bytes(int64_t num_rows, int64_t vocab, int to
 int npd_top_k_sample(int64_t *out_ids, const void *logits, const float *uniforms, int64_t num_rows,
                      int64_t vocab, int64_t row_stride, int top_k, int dtype, void *workspace,
                      int64_t workspace_bytes, void *stream);
+
+/* ---- (7) paged decode attention with shaped scores --------------------------------------
+ * No counterpart in the reference.  npd_paged_decode_attention with the scores changed before
+ * the softmax: for the query of sequence s, at position n - 1 with n = seq_lens[s], and key j,
+ *   x = scale * q . k_j
+ *   x = score_cap * tanh(x / score_cap)          when score_cap > 0 (0 = scores are not capped)
+ *   x = x - distance_slopes[h] * (n - 1 - j)     when distance_slopes (device float32 [num_q_heads]) is not NULL
+ * over the keys max(0, n - window) <= j < n       (window 0 = all keys of the sequence).
+ * Pages wholly before the window are not read, and neither are their block-table entries: they
+ * may name pages that belong to someone else by now.  What the page slots before the window and
+ * behind the sequence hold (NaN included) does not reach the result.  A sequence with
+ * seq_lens[s] == 0 gets a zero row.  Shapes and layouts as in npd_paged_decode_attention, the
+ * interleaved layouts excepted; `flags` takes NPD_FLAG_MAX_CTAS.  score_cap must be 0
+ * or between 1e-30 and 1e38, window not negative.  `workspace`: npd_decode_workspace_bytes(...) bytes,
+ * zeroed once, as there; a launch leaves its tickets at zero.  `status` (device int32, may be
+ * NULL) receives the NPD_STATUS_* bits; when NULL the workspace's first word does.          */
+int npd_paged_scored_attention(void *out, const void *q, const void *k_cache, const void *v_cache,
+                               const int32_t *block_tables, const int32_t *seq_lens, float scale,
+                               float score_cap, const float *distance_slopes, int64_t window,
+                               int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads,
+                               int64_t head_dim, int64_t block_size, int64_t max_blocks_per_seq,
+                               int64_t num_blocks, int64_t cache_block_stride, int64_t bt_row_stride,
+                               int dtype, void *workspace, size_t workspace_bytes, int32_t *status,
+                               int flags, void *stream);
+
+/* ---- (10) the norms between two blocks of a layer, with gate and residual sum -------------
+ * No counterpart in the reference (its model's modules run one after the other).  Per row:
+ *   y = x;   y = y * rsqrt(mean(y^2) + eps) * (post_weight + weight_offset)   unless post_weight is NULL
+ *   y = gate * y                                                              unless gate is NULL
+ *   r = residual + residual_scale * y                                         -> residual_out
+ *   h = r * rsqrt(mean(r^2) + eps) * (weight + weight_offset)                 -> out
+ * in fp32, residual_out and out rounded once each (h is computed from the unrounded r).
+ * Rows are `hidden` contiguous elements, `*_row_stride` elements apart; gate_row_stride 0 = one
+ * gate row for all.  f16 / bf16 / f32, all tensors of one type; hidden a multiple of 8 up to
+ * NPD_NORMS_MAX_HIDDEN; pointers and strides multiples of 16 bytes.  residual_out and out may
+ * each be x or residual (the same rows at the same stride); no other overlap.               */
+#define NPD_NORMS_MAX_HIDDEN 32768
+int npd_residual_norms(void *residual_out, void *out, const void *x, const void *residual,
+                       const void *weight, const void *post_weight, const void *gate,
+                       float residual_scale, float eps, float weight_offset, int64_t num_rows,
+                       int64_t hidden, int64_t x_row_stride, int64_t residual_row_stride,
+                       int64_t gate_row_stride, int64_t residual_out_row_stride,
+                       int64_t out_row_stride, int dtype, void *stream);
 
 /* Enables peer access from the current device to `peer_device` (idempotent).
  * Stands in for the driver-side mapping torch's copy_ sets up in the reference

@@ -17,8 +17,8 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libnanopd_b200.so"
 SOURCES = ["capi.cu", "kv_store.cu", "decode_attention.cu", "prefill_attention.cu", "kv_migrate.cu",
-           "qk_rope_store.cu", "top_k_sample.cu"]
-HEADERS = [CSRC / "npd_common.cuh", PKG_DIR.parent / "include" / "nanopd_b200.h",
+           "qk_rope_store.cu", "top_k_sample.cu", "scored_attention.cu", "residual_norms.cu"]
+HEADERS = [CSRC / "npd_common.cuh", CSRC / "decode_kernel.cuh", CSRC / "prefill_kernel.cuh", PKG_DIR.parent / "include" / "nanopd_b200.h",
            PKG_DIR.parent / "include" / "nanopd_b200_testing.h"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -26,10 +26,10 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
     "-cudart", "static",
 ]
-# --use_fast_math only where it was measured to pay and no result is pinned bit for bit against a library: the two
+# --use_fast_math only where it was measured to pay and no result is pinned bit for bit against a library: the
 # attention kernels (their exponentials are explicit ex2.approx anyway).  The sampler's softmax and the norm/rotary
 # kernel are compared with torch / transformers element by element and keep IEEE division, expf and sqrt.
-FAST_MATH_SOURCES = {"decode_attention.cu", "prefill_attention.cu"}
+FAST_MATH_SOURCES = {"decode_attention.cu", "prefill_attention.cu", "scored_attention.cu"}
 
 
 def _nvcc() -> str:

@@ -2,7 +2,7 @@
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p, POINTER
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnanopd_b200.so"
@@ -18,6 +18,7 @@ SIGNATURES = {
     "npd_version": (c_int, []),
     "npd_last_error": (c_char_p, []),
     "npd_read_status": (c_int, [c_void_p, POINTER(c_int32), c_void_p]),
+    "npd_capture_id": (c_int, [c_void_p, POINTER(c_uint64)]),
     "npd_kv_store": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                              c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                              c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
@@ -45,6 +46,9 @@ SIGNATURES = {
     "npd_top_k_sample_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "npd_top_k_sample": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p,
                                  c_int64, c_void_p]),
+    "npd_paged_scored_attention": (c_int, [c_void_p] * 6 + [c_float, c_float, c_void_p] + [c_int64] * 10 +
+                                   [c_int, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
+    "npd_residual_norms": (c_int, [c_void_p] * 7 + [c_float] * 3 + [c_int64] * 7 + [c_int, c_void_p]),
     "npd_enable_peer_access": (c_int, [c_int]),
 }
 

@@ -3,6 +3,7 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "npd_common.cuh"
 
@@ -80,6 +81,16 @@ int encode_cache_tensor_map(CUtensorMap *map, const void *base, int dtype, int64
     return encode_tiled_3d(map, base, dtype, dims, strides, box);
 }
 
+int check_score_shape(const char *op, float scale, float score_cap, const float *distance_slopes, int64_t window) {
+    const float cap_in = score_cap > 0.f ? 2.f * 1.4426950408889634f * scale / score_cap : 0.f;
+    NPD_REQUIRE(std::isfinite(score_cap) && (score_cap == 0.f || score_cap >= 1e-30f) && std::isfinite(cap_in) && std::isfinite(score_cap * 1.5f),
+                NPD_ERR_INVALID_ARG, "%s: the score cap must be 0 (none) or between 1e-30 and 1e38", op);
+    NPD_REQUIRE(window >= 0, NPD_ERR_INVALID_ARG, "%s: the window must not be negative (0 = none)", op);
+    NPD_REQUIRE((reinterpret_cast<uintptr_t>(distance_slopes) & 3u) == 0, NPD_ERR_INVALID_ARG,
+                "%s: distance_slopes must be 4-byte aligned", op);
+    return NPD_OK;
+}
+
 }  // namespace npd
 
 extern "C" {
@@ -94,6 +105,15 @@ int npd_read_status(int32_t *status_dev, int32_t *out, void *stream) {
     NPD_CUDA_TRY(cudaMemcpyAsync(out, status_dev, sizeof(int32_t), cudaMemcpyDeviceToHost, st));
     NPD_CUDA_TRY(cudaMemsetAsync(status_dev, 0, sizeof(int32_t), st));
     NPD_CUDA_TRY(cudaStreamSynchronize(st));
+    return NPD_OK;
+}
+
+int npd_capture_id(void *stream, uint64_t *id) {
+    NPD_REQUIRE(id != nullptr, NPD_ERR_INVALID_ARG, "npd_capture_id: NULL pointer");
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long found = 0;
+    NPD_CUDA_TRY(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &found));
+    *id = status == cudaStreamCaptureStatusActive ? found : 0;
     return NPD_OK;
 }
 

@@ -65,6 +65,9 @@ int encode_cache_tensor_map(CUtensorMap *map, const void *base, int dtype, int64
                             int64_t rows_per_block, int64_t num_blocks,
                             int64_t block_stride_elems, int box_rows);
 
+// Checks of the arguments that shape scores, the same for decode and prompts.
+int check_score_shape(const char *op, float scale, float score_cap, const float *distance_slopes, int64_t window);
+
 }  // namespace npd
 
 // ---------------------------------------------------------------------------

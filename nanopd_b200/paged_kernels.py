@@ -14,6 +14,7 @@ the kernels skip the access and set a status word that :func:`check_status` read
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 from typing import Dict, Optional, Sequence, Tuple
 
@@ -65,8 +66,15 @@ def release_workspaces(device=None) -> None:
         keys = [k for k in _workspaces if idx is None or k[0] == idx]
         for d in {k[0] for k in keys}:
             torch.cuda.synchronize(d)
+        scratch_keys = [k for k in _scratch if idx is None or k[0] == idx]
+        for d in {k[0] for k in scratch_keys} - {k[0] for k in keys}:
+            torch.cuda.synchronize(d)
         for k in keys:
             del _workspaces[k]
+        for k in scratch_keys:
+            del _scratch[k]
+        for k in [k for k in _captured_scratch if idx is None or k[0] == idx]:
+            del _captured_scratch[k]           # the graph's own pool keeps the memory
 
 
 def check_status(device=None, raise_on_error: bool = True) -> int:
@@ -87,6 +95,18 @@ def check_status(device=None, raise_on_error: bool = True) -> int:
             bits |= out.value
             if out.value & _lib.NPD_STATUS_WAIT_TIMEOUT:
                 ws.zero_()          # a launch that gave up may have left arrival tickets behind
+                torch.cuda.synchronize(idx)
+        word = _status_words.get(idx)
+        if word is not None:
+            torch.cuda.synchronize(idx)         # any stream may have set it
+            seen = int(word[0].item())
+            if seen:
+                bits |= seen
+                word.zero_()
+                if seen & _lib.NPD_STATUS_WAIT_TIMEOUT:
+                    for k, ws in list(_scratch.items()):
+                        if k[0] == idx:
+                            ws.zero_()
                 torch.cuda.synchronize(idx)
     if bits and raise_on_error:
         names = [n for n, b in (("bad block id", 1), ("bad position / seq_len", 2), ("wait time-out", 4)) if bits & b]
@@ -143,6 +163,55 @@ def _ws_ptr(dev_index: int, handle: int, nbytes: int):
     ws = _workspaces.get((dev_index, handle))
     if ws is None or ws.numel() < nbytes:
         ws = _workspace(torch.device("cuda", dev_index), handle, nbytes)
+    return ws
+
+
+# ---------------------------------------------------------------------------
+# Scratch of the operators below (scored and shared-prefix attention).  Eager calls share one buffer per device and
+# stream.  A call that is being captured takes scratch that belongs to its capture (allocated from the graph's own
+# pool, cleared by a node of the graph): two graphs captured on one stream may then be replayed side by side.  The
+# status bits of all of them go to one word per device, which lives as long as the process.
+# ---------------------------------------------------------------------------
+_scratch: Dict[Tuple[int, int], torch.Tensor] = {}
+_captured_scratch: Dict[Tuple[int, int], Tuple[int, torch.Tensor, int]] = {}     # the stream's latest capture; bytes cleared
+_status_words: Dict[int, torch.Tensor] = {}
+
+
+def _status_ptr(dev_index: int) -> int:
+    word = _status_words.get(dev_index)
+    if word is None:
+        _require(not torch.cuda.is_current_stream_capturing(),
+                 "call the operator once on this device before capturing it (it allocates its status word on first use)")
+        with _ws_lock:
+            word = _status_words.get(dev_index)
+            if word is None:
+                made = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", dev_index))
+                torch.cuda.synchronize(dev_index)            # other streams may write it from now on
+                _status_words[dev_index] = word = made
+    return word.data_ptr()
+
+
+def _scratch_for(dev_index: int, handle: int, nbytes: int, cleared: int) -> torch.Tensor:
+    """At least ``nbytes`` of scratch for a call on the current stream (``handle``), the first ``cleared`` bytes zero when
+    it is first used."""
+    key = (dev_index, handle)
+    if torch.cuda.is_current_stream_capturing():
+        capture = ctypes.c_uint64(0)
+        _lib.check(_C.npd_capture_id(handle, ctypes.byref(capture)))
+        held = _captured_scratch.get(key)
+        if held is None or held[0] != capture.value or held[1].numel() < nbytes:
+            ws, before = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev_index)), 0
+        else:
+            ws, before = held[1], held[2]
+        if before < cleared:
+            ws[before:cleared].zero_()
+            with _ws_lock:
+                _captured_scratch[key] = (capture.value, ws, cleared)
+        return ws
+    ws = _scratch.get(key)
+    if ws is None or ws.numel() < nbytes:
+        with _ws_lock:
+            _scratch[key] = ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev_index))
     return ws
 
 
@@ -459,6 +528,83 @@ def paged_prefill_attention(out, query, key_cache, value_cache, block_tables,
             nchunks, float(scale), hq, hkv, d, bs, max_blk, nb, cstride, block_tables.stride(0),
             _DTYPE_CODE[query.dtype], ws.data_ptr(), ws.numel(),
             int(_flags) | ((int(max_ctas) & 0xffff) << 8), handle))
+
+
+# ---------------------------------------------------------------------------
+# (2c) decode attention with shaped scores
+# ---------------------------------------------------------------------------
+_scored_plans: Dict[tuple, tuple] = {}
+
+
+def _score_shape(name: str, score_cap, distance_slopes, window, hq: int, dev) -> None:
+    _require(distance_slopes is None or (distance_slopes.dtype == torch.float32 and distance_slopes.device == dev
+                                         and distance_slopes.shape == (hq,) and distance_slopes.stride(0) == 1),
+             f"{name}: distance_slopes must be a contiguous float32 [num_heads] tensor on the query's device")
+    _require(int(window) == window and 0 <= window < 2 ** 31, f"{name}: window must be a whole number, 0 for none")
+    _require(math.isfinite(score_cap) and score_cap >= 0, f"{name}: score_cap must be finite and not negative, 0 for none")
+
+
+def _check_single_token_call(name: str, out, query, key_cache, value_cache, block_tables, seq_lens, block_size, max_num_blocks_per_seq):
+    """The checks that the operators for one query token per sequence share; returns
+    (device, S, hq, hkv, d, block, blocks, cache stride, table width, table row stride)."""
+    _require(query.is_cuda and query.dim() == 3, f"{name}: query must be a CUDA tensor [num_seqs, num_heads, head_size]")
+    dev = query.device
+    S, hq, d = query.shape
+    _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and query.is_contiguous() and out.is_contiguous(),
+             f"{name}: out must match query in shape, dtype and device; both contiguous")
+    _require(query.dtype in (torch.float16, torch.bfloat16), f"{name} supports float16 and bfloat16, got {query.dtype}")
+    _require(block_tables.dtype == torch.int32 and seq_lens.dtype == torch.int32, f"{name}: block_tables and seq_lens must be int32")
+    _require(key_cache.dtype == query.dtype == value_cache.dtype and all(t.device == dev for t in (key_cache, value_cache, block_tables, seq_lens)),
+             f"{name}: caches and tables must match query's dtype and device")
+    nb, hkv, bs, cd, cstride = _cache_geometry(key_cache, "key_cache")
+    _require(_cache_geometry(value_cache, "value_cache") == (nb, hkv, bs, cd, cstride), "key_cache and value_cache layouts differ")
+    _require(cd == d, "head_size of query and cache differ")
+    _require(int(block_size) == bs, f"block_size argument {block_size} != cache block size {bs}")
+    _require(hq % hkv == 0, "num_heads must be a multiple of num_kv_heads")
+    _require(seq_lens.dim() == 1 and seq_lens.numel() == S and (S < 2 or seq_lens.stride(0) == 1), "seq_lens must be contiguous [S]")
+    max_blk = int(max_num_blocks_per_seq)
+    _require(block_tables.dim() == 2 and block_tables.size(0) == S, f"{name}: block_tables must be [num_seqs, max_blocks]")
+    _require(1 <= max_blk <= block_tables.size(1), "max_num_blocks_per_seq out of range")
+    _require(block_tables.stride(1) == 1 or block_tables.size(1) == 1, f"{name}: block_tables rows must be contiguous")
+    row_stride = block_tables.stride(0) if S > 1 else block_tables.size(1)
+    return dev, S, hq, hkv, d, bs, nb, cstride, max_blk, row_stride
+
+
+def paged_scored_attention(out, query, key_cache, value_cache, block_tables, seq_lens, scale: float, block_size: int,
+                           max_num_blocks_per_seq: int, score_cap: float = 0.0, distance_slopes=None, window: int = 0,
+                           max_ctas: int = 0) -> None:
+    """:func:`paged_attention_forward` with the scores shaped before the softmax, written in place.
+
+    For the query of sequence ``s``, at position ``n - 1`` with ``n = seq_lens[s]``, and key ``j``:
+    ``x = scale * q . k_j``; with ``score_cap > 0`` ``x = score_cap * tanh(x / score_cap)``; with ``distance_slopes`` (float32
+    ``[num_heads]``) ``x -= distance_slopes[h] * (n - 1 - j)``; over the keys ``max(0, n - window) <= j < n``, all of them with
+    ``window == 0``.  Pages wholly before the window are not read and their table entries may be stale.  A sequence of length 0
+    gets a zero row.  ``block_tables`` is int32 ``[S, >= max_num_blocks_per_seq]`` with contiguous rows; the other arguments are
+    those of :func:`paged_attention_forward` (the interleaved layouts are not taken).
+    """
+    try:
+        key = (_sig(out, query, key_cache, value_cache, block_tables, seq_lens), block_size, max_num_blocks_per_seq,
+               None if distance_slopes is None else _sig(distance_slopes), score_cap, window, max_ctas)
+        plan = _scored_plans.get(key)
+    except (AttributeError, TypeError):
+        raise RuntimeError("paged_scored_attention takes tensors and numbers") from None
+    if plan is None:
+        dev, S, hq, hkv, d, bs, nb, cstride, max_blk, row_stride = _check_single_token_call(
+            "paged_scored_attention", out, query, key_cache, value_cache, block_tables, seq_lens, block_size, max_num_blocks_per_seq)
+        _score_shape("paged_scored_attention", score_cap, distance_slopes, window, hq, dev)
+        _require(0 <= int(max_ctas) <= 0xffff, "max_ctas out of range")
+        if S == 0:
+            return
+        need = _C.npd_decode_workspace_bytes(S, hq, hkv, d, dev.index)
+        plan = (dev.index, need, 256 + 4 * S * hq, int(max_ctas) << 8, float(score_cap), int(window),
+                (S, hq, hkv, d, bs, max_blk, nb, cstride, row_stride, _DTYPE_CODE[query.dtype]))
+        _remember(_scored_plans, key, plan)
+    dev_index, need, cleared, flags, cap, win, args = plan
+    handle = _raw_stream(dev_index)
+    ws = _scratch_for(dev_index, handle, need, min(cleared, need))
+    _call(dev_index, _C.npd_paged_scored_attention, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+          block_tables.data_ptr(), seq_lens.data_ptr(), float(scale), cap, None if distance_slopes is None else distance_slopes.data_ptr(), win,
+          *args, ws.data_ptr(), ws.numel(), _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
