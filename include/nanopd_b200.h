@@ -260,6 +260,52 @@ int npd_paged_scored_attention(void *out, const void *q, const void *k_cache, co
                                int dtype, void *workspace, size_t workspace_bytes, int32_t *status,
                                int flags, void *stream);
 
+/* ---- (8) chunked-prefill attention with shaped scores ------------------------------------
+ * npd_paged_prefill_attention with the scores of (7): a query at position i sees the keys
+ * max(0, i - window + 1) <= j <= i (window 0 = all up to i), its distance to key j is i - j.
+ * Pages wholly before the window of a chunk's first query are not read.  `workspace`:
+ * npd_prefill_workspace_bytes(...) bytes, zeroed once; `status`, `flags` as in (7).          */
+int npd_paged_scored_prefill_attention(void *out, const void *q, const void *k_cache,
+                                       const void *v_cache, const int32_t *block_tables,
+                                       const int32_t *chunk_q_offset_host,
+                                       const int32_t *chunk_tokens_host,
+                                       const int32_t *chunk_start_host, int64_t num_chunks,
+                                       float scale, float score_cap, const float *distance_slopes,
+                                       int64_t window, int64_t num_q_heads, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t block_size,
+                                       int64_t max_blocks_per_seq, int64_t num_blocks,
+                                       int64_t cache_block_stride, int64_t bt_row_stride, int dtype,
+                                       void *workspace, size_t workspace_bytes, int32_t *status,
+                                       int flags, void *stream);
+
+/* ---- (9) decode attention for a batch that shares prefixes --------------------------------
+ * No counterpart in the reference.  The result of npd_paged_decode_attention, computed with the
+ * pages that several sequences share read and multiplied once per group of sequences.
+ * Group g is the sequences group_offsets[g] <= s < group_offsets[g + 1] (device int32
+ * [num_groups + 1], ascending); their first shared_lens[g] tokens (device int32 [num_groups])
+ * lie in the same pages, that is, their table rows agree there.  Sequences outside every group,
+ * groups of one, and what a shared_len reaches beyond the shortest non-empty sequence of its
+ * group are attended to as in npd_paged_decode_attention.  Only whole tiles of 16 tokens are
+ * shared; the rest of a prefix is read per sequence.  The lengths, offsets and tables are read on
+ * the device: they may change between replays of a captured call.  Offsets that are not
+ * ascending within [0, num_seqs] and negative shared_lens raise NPD_STATUS_BAD_POSITION and
+ * share nothing.  num_groups between 1 and 4096, num_q_heads/num_kv_heads <= 128; other shapes
+ * as in (2), without the interleaved layouts; `status` and `flags` as in (7).  `workspace`:
+ * npd_shared_prefix_workspace_bytes(...) bytes, 256-byte aligned, zeroed once; two calls that may
+ * overlap on the GPU need two workspaces.                                                   */
+size_t npd_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t num_q_heads,
+                                         int64_t num_kv_heads, int64_t head_dim, int device);
+int npd_paged_shared_prefix_attention(void *out, const void *q, const void *k_cache,
+                                      const void *v_cache, const int32_t *block_tables,
+                                      const int32_t *seq_lens, const int32_t *group_offsets,
+                                      const int32_t *shared_lens, float scale, int64_t num_seqs,
+                                      int64_t num_groups, int64_t num_q_heads, int64_t num_kv_heads,
+                                      int64_t head_dim, int64_t block_size,
+                                      int64_t max_blocks_per_seq, int64_t num_blocks,
+                                      int64_t cache_block_stride, int64_t bt_row_stride, int dtype,
+                                      void *workspace, size_t workspace_bytes, int32_t *status,
+                                      int flags, void *stream);
+
 /* ---- (10) the norms between two blocks of a layer, with gate and residual sum -------------
  * No counterpart in the reference (its model's modules run one after the other).  Per row:
  *   y = x;   y = y * rsqrt(mean(y^2) + eps) * (post_weight + weight_offset)   unless post_weight is NULL

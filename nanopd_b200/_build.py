@@ -17,8 +17,10 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libnanopd_b200.so"
 SOURCES = ["capi.cu", "kv_store.cu", "decode_attention.cu", "prefill_attention.cu", "kv_migrate.cu",
-           "qk_rope_store.cu", "top_k_sample.cu", "scored_attention.cu", "residual_norms.cu"]
-HEADERS = [CSRC / "npd_common.cuh", CSRC / "decode_kernel.cuh", CSRC / "prefill_kernel.cuh", PKG_DIR.parent / "include" / "nanopd_b200.h",
+           "qk_rope_store.cu", "top_k_sample.cu", "scored_attention.cu", "scored_prefill.cu",
+           "shared_prefix.cu", "prefix_pass.cu", "residual_norms.cu"]
+HEADERS = [CSRC / "npd_common.cuh", CSRC / "decode_kernel.cuh", CSRC / "prefill_kernel.cuh",
+           CSRC / "shared_prefix.cuh", PKG_DIR.parent / "include" / "nanopd_b200.h",
            PKG_DIR.parent / "include" / "nanopd_b200_testing.h"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -29,7 +31,8 @@ NVCC_FLAGS = [
 # --use_fast_math only where it was measured to pay and no result is pinned bit for bit against a library: the
 # attention kernels (their exponentials are explicit ex2.approx anyway).  The sampler's softmax and the norm/rotary
 # kernel are compared with torch / transformers element by element and keep IEEE division, expf and sqrt.
-FAST_MATH_SOURCES = {"decode_attention.cu", "prefill_attention.cu", "scored_attention.cu"}
+FAST_MATH_SOURCES = {"decode_attention.cu", "prefill_attention.cu", "scored_attention.cu", "scored_prefill.cu",
+                     "shared_prefix.cu", "prefix_pass.cu"}
 
 
 def _nvcc() -> str:

@@ -48,6 +48,12 @@ SIGNATURES = {
                                  c_int64, c_void_p]),
     "npd_paged_scored_attention": (c_int, [c_void_p] * 6 + [c_float, c_float, c_void_p] + [c_int64] * 10 +
                                    [c_int, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
+    "npd_paged_scored_prefill_attention": (c_int, [c_void_p] * 5 + [POINTER(c_int32)] * 3 +
+                                           [c_int64, c_float, c_float, c_void_p] + [c_int64] * 9 +
+                                           [c_int, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
+    "npd_shared_prefix_workspace_bytes": (c_size_t, [c_int64] * 5 + [c_int]),
+    "npd_paged_shared_prefix_attention": (c_int, [c_void_p] * 8 + [c_float] + [c_int64] * 10 +
+                                          [c_int, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
     "npd_residual_norms": (c_int, [c_void_p] * 7 + [c_float] * 3 + [c_int64] * 7 + [c_int, c_void_p]),
     "npd_enable_peer_access": (c_int, [c_int]),
 }

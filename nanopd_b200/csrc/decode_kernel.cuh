@@ -34,6 +34,7 @@
 #include <cstdlib>
 
 #include "npd_common.cuh"
+#include "shared_prefix.cuh"
 
 namespace {
 
@@ -42,7 +43,6 @@ using namespace npd;
 constexpr int kTile = 16;               // tokens per stage
 constexpr int kMaxSeqsPerLaunch = 4096; // prefix array lives in shared memory
 constexpr int kMaxFloorTilesPerWorker = 16;   // upper end of the floor on tiles per worker (see tiles_per_worker)
-constexpr int kPrefixRows = 256;        // rows of one item of the prefix pass (two query tiles of 128)
 constexpr int kStatusBytes = 256;       // workspace header: status word + padding
 constexpr int kTicketCapacity = 1 << 18;   // ticket words (1 MiB): a FIXED region right after the header, so that no
                                         // launch shape ever puts partial records where another shape keeps tickets
@@ -75,9 +75,9 @@ struct DecodeParams {
     const float *slopes;  // [num_q_heads] slope of the distance bias, or nullptr
     int window;           // keys visible behind the query, its own included; INT32_MAX = all
     // kTail: what the prefix pass left (see shared_prefix.cu)
-    const struct PrefixSeqPlan *seq_plan;   // [num_seqs]
+    const PrefixSeqPlan *seq_plan;   // [num_seqs]
     int seq_base;                           // index of the launch's first sequence in the call's batch
-    const struct PrefixPlanHead *plan_head;
+    const PrefixPlanHead *plan_head;
     const float *prefix_o;        // [rows][D] normalised rows of the pieces
     const float *prefix_lse;      // [rows] log2 of the pieces' softmax sums, maximum included
     int num_kv_heads;             // physical
@@ -90,22 +90,6 @@ struct DecodeParams {
 //            a tile are four numbers a thread, so the tests cost nothing beside the tile's loads)
 //   kTail    softmax over the sequence's own pages behind a shared prefix, joined with the prefix pass's pieces
 enum : int { kPlain = 0, kScored = 1, kTail = 2 };
-
-// Written by the plan kernel of the shared-prefix attention, read by the prefix pass and by kTail.
-struct PrefixPlanHead {
-    int total_units;      // key tiles over all (group, query tiles, kv head) items
-    int units_per_worker;
-    int bad_groups;       // group_offsets were not ascending within [0, num_seqs]: nothing is shared
-    int pad;
-};
-struct PrefixSeqPlan {
-    int first_tile;       // 16-token tiles of the sequence that the prefix pass covers
-    int unit0;            // first unit of this sequence's item for kv head 0
-    int key_tiles;        // units of one item (0: nothing is shared)
-    int item_first_seq;   // first sequence of the item
-    int item_seqs;        // sequences of the item
-    int pad[3];
-};
 
 template <int MODE>
 __device__ __forceinline__ int first_visible(const DecodeParams &p, int len) {

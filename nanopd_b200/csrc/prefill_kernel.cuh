@@ -42,6 +42,7 @@
 #include <vector>
 
 #include "npd_common.cuh"
+#include "shared_prefix.cuh"
 
 namespace {
 
@@ -80,6 +81,14 @@ constexpr int kTmemCols = 512;     // S_A | S_B | O_A | O_B, 128 columns each; a
 constexpr float kRescaleThreshold = 8.f;   // log2 units: O is rescaled only when a row max grows by more
 constexpr long long kWaitCycles = 4000000000LL;
 
+// What the kernel computes (template parameter MODE):
+//   kCausal  prompt chunks, plain causal attention
+//   kShaped  prompt chunks with capped scores, a distance bias and a sliding window (each optional)
+//   kPrefix  a decode batch's queries over the shared prefix of their group: every key of a piece of the prefix is visible
+//            to every row, and the rows leave as fp32 with their log2 sums, to be joined with the rest of each sequence.
+//            A CTA takes an equal run of (group, query tiles, kv head, key tile) units, cut where items end.
+enum : int { kCausal = 0, kShaped = 1, kPrefix = 2 };
+
 struct PrefillParams {
     void *out;
     const int32_t *block_tables;
@@ -98,6 +107,18 @@ struct PrefillParams {
     int chunk_q_offset[kMaxChunks];
     int chunk_tokens[kMaxChunks];
     int chunk_start[kMaxChunks];
+    // kShaped; the score in the log2 domain is y * R(y^2) with y = 2 scale/cap * (q . k) below |y| = 2 (R: cap_poly), and
+    // cap_log2 - 2 cap_log2 / (1 + e^y) elsewhere (y = 2z: tanh z = 1 - 2 / (1 + e^2z))
+    float cap_y;                      // 2 * scale / cap; 0 = scores are not capped
+    float cap_log2;                   // cap * log2(e)
+    float cap_poly[6];
+    const float *slopes;              // [num_q_heads] or nullptr
+    int window;                       // keys visible behind a query, its own included; INT32_MAX = all
+    // kPrefix
+    const PrefixGroup *groups;
+    const PrefixSeed *seeds;          // [gridDim.x]
+    const PrefixPlanHead *plan;
+    float *prefix_o, *prefix_lse;
     int num_pairs;                    // entries of pair_order
     int *work_counter;                // two device int32, zero before the launch and put back to zero by its last
                                       // CTA: [0] items handed out beyond the first gridDim.x, [1] CTAs that have left
@@ -223,6 +244,67 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     return d;
 }
 
+// Shapes the 64 raw scores of a row's half-step in place (cap, distance bias), into the log2 domain; `rel` is the first
+// key's position relative to the query's.  Returns what is still to be added to each of them, the bias of the first key.
+// The cap: tanh(z) = z P(z^2) on |z| < 1, P of degree 5 fitted by Remez exchange for the least relative error (6e-7);
+// y = 2z carries the test for it: an exponent of 128 or more, that is |y| >= 2, an infinity or a NaN, sets bit 30, and one
+// OR over the row finds it.  Scores as large as the cap are rare (a cap tames the rare ones), so the warp's test almost
+// never takes the second branch, an exponential and a reciprocal per score: three special-function results a score would
+// bound the kernel (8192 scores per query tile and half-step at 16 a clock are 1536 clocks; the two products take 512).
+__device__ __forceinline__ float shape_scores(float (&sc)[2][32], float slope2, int rel, const PrefillParams &p) {
+    if (p.cap_y != 0.f) {
+        const float2 c2 = make_float2(p.cap_y, p.cap_y);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float2 y = __fmul2_rn(make_float2(sc[cc][i], sc[cc][i + 1]), c2);
+                sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
+                bits |= __float_as_uint(y.x) | __float_as_uint(y.y);
+            }
+        if (__any_sync(0xffffffffu, (bits & 0x40000000u) != 0)) {
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    sc[cc][i] = p.cap_log2 - __fdividef(2.f * p.cap_log2, 1.f + fast_exp2(sc[cc][i] * 1.4426950408889634f));
+        } else {
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 y = make_float2(sc[cc][i], sc[cc][i + 1]), w = __fmul2_rn(y, y);
+                    float2 q = make_float2(p.cap_poly[5], p.cap_poly[5]);
+#pragma unroll
+                    for (int k = 4; k >= 0; --k) q = __ffma2_rn(q, w, make_float2(p.cap_poly[k], p.cap_poly[k]));
+                    q = __fmul2_rn(q, y);
+                    sc[cc][i] = q.x, sc[cc][i + 1] = q.y;
+                }
+        }
+    } else {
+        const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float2 y = __fmul2_rn(make_float2(sc[cc][i], sc[cc][i + 1]), c2);
+                sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
+            }
+    }
+    if (p.slopes == nullptr) return 0.f;
+    const float2 s2 = make_float2(slope2, slope2);
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float2 y = __ffma2_rn(make_float2(static_cast<float>(cc * 32 + i), static_cast<float>(cc * 32 + i + 1)), s2,
+                                        make_float2(sc[cc][i], sc[cc][i + 1]));
+            sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
+        }
+    return slope2 * static_cast<float>(rel);
+}
+
 // Shared-memory matrix descriptors (version 1, 128-byte swizzle, 8-row groups 1024 B apart).
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
@@ -285,11 +367,24 @@ struct Item {
     int ntiles[2];          // K/V tiles of 128 keys they lie in
     int n_kv;
 };
+// kShaped and kPrefix walk the K/V tiles from t0 on (Item counts half-steps and tiles from there).
+struct ItemFrom : Item {
+    int t0;
+    int lo;                 // kShaped: first key that any row of the item sees
+    int row0;               // kPrefix: first row of the piece's records
+};
+template <int MODE> struct ItemOf { using type = ItemFrom; };
+template <> struct ItemOf<kCausal> { using type = Item; };
+template <int MODE> __device__ __forceinline__ int item_t0(const typename ItemOf<MODE>::type &it) {
+    if constexpr (MODE == kCausal) return 0;
+    else return it.t0;
+}
 
-struct alignas(8) SmemCtrl {
+template <typename ItemT>
+struct alignas(8) SmemCtrlT {
     uint64_t sched_full[kSchedSlots];   // the producer warp has published the next work item
     int sched_item[kSchedSlots];
-    Item sched_desc[kSchedSlots];       // the published item, decoded once by the producer warp: the other roles'
+    ItemT sched_desc[kSchedSlots];      // the published item, decoded once by the producer warp: the other roles'
                                         // way from one item to the next stays a few loads (their decoding it
                                         // themselves — divisions, indexed kernel parameters, cold code — took a
                                         // softmax group ~2500 clocks per item)
@@ -311,9 +406,12 @@ struct alignas(8) SmemCtrl {
 };
 
 
+using SmemCtrl = SmemCtrlT<ItemFrom>;       // the larger one: what the launcher reserves
+
 // Work item `item` = kv head (item % Hkv) of entry (item / Hkv) of the host-sorted pair list.
-__device__ __forceinline__ Item decode_item(const PrefillParams &p, int item) {
-    Item it;
+template <int MODE>
+__device__ __forceinline__ typename ItemOf<MODE>::type decode_item(const PrefillParams &p, int item) {
+    typename ItemOf<MODE>::type it;
     it.h = item % p.num_kv_heads;
     const uint32_t entry = p.pair_order[item / p.num_kv_heads];
     const int c = static_cast<int>(entry >> 16), pair = static_cast<int>(entry & 0xffffu);
@@ -322,16 +420,69 @@ __device__ __forceinline__ Item decode_item(const PrefillParams &p, int item) {
     it.start = p.chunk_start[c];
     it.qoff = p.chunk_q_offset[c];
     it.ctx_end = it.start + n_tok;                              // keys written so far for this sequence
+    int skipped = 0;                                            // half-steps in front of the first tile walked
+    if constexpr (MODE == kShaped) {
+        const long long lo = (long long)it.start + p.query_tiles * pair * p.tq - p.window + 1;   // of the item's first query
+        it.lo = lo > 0 ? static_cast<int>(lo) : 0;
+        it.t0 = it.lo / (kHalfKeys * p.half_steps_per_tile);
+        it.row0 = 0;
+        skipped = it.t0 * p.half_steps_per_tile;
+    }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         it.tok0[x] = (p.query_tiles * pair + x) * p.tq;
         it.tq_valid[x] = x < p.query_tiles ? max(0, min(p.tq, n_tok - it.tok0[x])) : 0;
         // keys [0, start + tok0 + tq_valid) are visible to the tile
-        it.nhalf[x] = it.tq_valid[x] > 0 ? (it.start + it.tok0[x] + it.tq_valid[x] + kHalfKeys - 1) / kHalfKeys : 0;
+        it.nhalf[x] = it.tq_valid[x] > 0 ? (it.start + it.tok0[x] + it.tq_valid[x] + kHalfKeys - 1) / kHalfKeys - skipped : 0;
         it.ntiles[x] = (it.nhalf[x] + p.half_steps_per_tile - 1) / p.half_steps_per_tile;
     }
     it.n_kv = max(it.ntiles[0], it.ntiles[1]);
     return it;
+}
+
+// kPrefix: the next piece of this CTA's run of units; false when the run is over.
+struct PrefixRun {
+    PrefixSeed at;
+    int left;
+};
+__device__ __forceinline__ bool prefix_item(const PrefillParams &p, PrefixRun &run, ItemFrom &it) {
+    if (run.left <= 0) return false;
+    PrefixGroup g = p.groups[run.at.group];
+    const int item_seqs = p.query_tiles * p.tq;
+    if (run.at.tile == g.key_tiles) {                           // step to the next item
+        run.at.tile = 0;
+        if (++run.at.head == p.num_kv_heads) {
+            run.at.head = 0;
+            ++run.at.pair;
+            if (run.at.pair * item_seqs >= g.seqs) {
+                run.at.pair = 0;
+                do g = p.groups[++run.at.group];                // units are left, so a group with some follows
+                while (g.key_tiles == 0);
+            }
+        }
+    }
+    const int tile_keys = kHalfKeys * p.half_steps_per_tile;
+    const int n = min(g.key_tiles - run.at.tile, run.left);
+    it.c = g.begin;                                             // the first sequence's table row names the shared pages
+    it.h = run.at.head;
+    it.start = 0;
+    it.qoff = g.begin;
+    it.t0 = run.at.tile;
+    it.lo = 0;
+    it.ctx_end = min(g.tokens, (run.at.tile + n) * tile_keys);
+    const int first = run.at.pair * item_seqs, seqs = min(item_seqs, g.seqs - first);
+    it.row0 = (g.begin + first) * p.num_q_heads + it.h * seqs * p.group;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        it.tok0[x] = first + x * p.tq;
+        it.tq_valid[x] = x < p.query_tiles ? max(0, min(p.tq, g.seqs - it.tok0[x])) : 0;
+        it.nhalf[x] = it.tq_valid[x] > 0 ? (it.ctx_end - it.t0 * tile_keys + kHalfKeys - 1) / kHalfKeys : 0;
+        it.ntiles[x] = it.tq_valid[x] > 0 ? n : 0;
+    }
+    it.n_kv = n;
+    run.at.tile += n;
+    run.left -= n;
+    return true;
 }
 
 // Persistent kernel: one CTA per SM.  Work items are handed out heaviest first through an atomic counter (the
@@ -344,7 +495,7 @@ __device__ __forceinline__ Item decode_item(const PrefillParams &p, int item) {
 // memory is the same).  A template parameter because the producer warps share their sub-partitions' issue slots
 // with two softmax warps each, and every instruction they run per key tile shows in the kernel's time (the
 // run-time form of this choice cost 2.3 %).
-template <typename T, int kD, int kBoxRows>
+template <typename T, int kD, int kBoxRows, int MODE = kCausal>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap tm_q,
                      const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
@@ -361,7 +512,9 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
     uint8_t *q_tiles = sbase;                                   // query tiles A and B
     uint8_t *k_ring = q_tiles + kQueryTiles * kQTileBytes;      // kStagesK K tiles
     uint8_t *v_ring = k_ring + kStagesK * kKvTileBytes;         // kStagesV V tiles
-    SmemCtrl *ctrl = reinterpret_cast<SmemCtrl *>(v_ring + kStagesV * kKvTileBytes);
+    using ItemT = typename ItemOf<MODE>::type;
+    using Ctrl = SmemCtrlT<ItemT>;
+    Ctrl *ctrl = reinterpret_cast<Ctrl *>(v_ring + kStagesV * kKvTileBytes);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int total_items = p.num_pairs * p.num_kv_heads;
@@ -448,12 +601,20 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         int stage = 0, round = 0;                               // ring position of the next tile
         NPD_TRACE_DECL
         bool ok = true;
+        PrefixRun run{};
+        if (MODE == kPrefix && k_role) {
+            run.at = p.seeds[blockIdx.x];
+            run.left = min(p.plan->units_per_worker, p.plan->total_units - static_cast<int>(blockIdx.x) * p.plan->units_per_worker);
+        }
         for (int k = 0; ok; ++k) {
             // Warp 8 fetches and publishes the next work item; warp 11 reads it like the other roles.  A slot is
             // reused kSchedSlots items later; by then every role has long read it (warp 8 cannot run more than
             // two items ahead of the MMA warps, which cannot run ahead of the V tiles or the softmax groups).
             int item = 0;
-            if (k_role) {
+            ItemT it;
+            if (MODE == kPrefix && k_role) {
+                if constexpr (MODE == kPrefix) item = prefix_item(p, run, it) ? 0 : -1;
+            } else if (k_role) {
                 if (lane == 0) {
                     // the first item of a CTA is its own index (no round trip to the counter before the first load);
                     // the counter hands out the items behind the first gridDim.x
@@ -465,9 +626,8 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 item = next_item(k, ok);
                 if (!__all_sync(0xffffffffu, ok)) break;
             }
-            Item it;
             if (k_role) {
-                if (item >= 0) it = decode_item(p, item);
+                if (MODE != kPrefix && item >= 0) it = decode_item<MODE>(p, item);
                 if (lane == 0) {
                     if (item >= 0) ctrl->sched_desc[k % kSchedSlots] = it;
                     *reinterpret_cast<volatile int *>(&ctrl->sched_item[k % kSchedSlots]) = item;
@@ -480,10 +640,13 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             }
             const int32_t *table = p.block_tables + (long long)it.c * p.bt_row_stride;
             // A box lies in one block: 16 keys of a block of 16 or 32, or all keys of a block of 8 or 4.
+            const int t0 = item_t0<MODE>(it);
             auto lookup = [&](int t, int i) {
-                const int key = t * kTK + gi[i] * 16 + sub[i] * kBoxRows;
+                const int key = (t0 + t) * kTK + gi[i] * 16 + sub[i] * kBoxRows;
                 int id = 0;
-                if (has_box[i] && t < it.n_kv && key < it.ctx_end) {
+                bool wanted = has_box[i] && t < it.n_kv && key < it.ctx_end;
+                if constexpr (MODE == kShaped) wanted = wanted && key + kBoxRows > it.lo;
+                if (wanted) {
                     id = __ldg(table + key / p.block_size);
                     if (id < 0 || id >= p.num_blocks) {
                         atomicOr(p.status, NPD_STATUS_BAD_BLOCK_ID);
@@ -496,7 +659,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
 #pragma unroll
             for (int i = 0; i < kIssues; ++i) id_next[i] = lookup(0, i);
             for (int t = 0; t < it.n_kv; ++t) {
-                const int key0 = t * kTK;
+                const int key0 = (t0 + t) * kTK;
                 int id[kIssues];
 #pragma unroll
                 for (int i = 0; i < kIssues; ++i) {
@@ -506,7 +669,10 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 // 16-key row groups holding at least one written key; the rest is never loaded
                 int ngroups = 0;
                 for (int g2 = 0; g2 < kTK / 16; ++g2) ngroups += (key0 + g2 * 16 < it.ctx_end) ? 1 : 0;
-                const uint32_t bytes = static_cast<uint32_t>(ngroups * kHalves * 16 * 128);
+                // boxes wholly before the window are not read either: their pages may have been given away
+                int skip = 0;                                   // keys of the tile in front of the first box read
+                if constexpr (MODE == kShaped) skip = max(0, it.lo - key0) / kBoxRows * kBoxRows;
+                const uint32_t bytes = static_cast<uint32_t>((ngroups * 16 - skip) * kHalves * 128);
                 // the stage is free once the MMAs that read the tile `stages` tiles back are done: the score MMAs
                 // for a K tile, the PV MMAs for a V tile
                 if (round > 0) ok = wait_or_abort(smem_u32(&empty[stage]), (round - 1) & 1, abort_flag, p.status);
@@ -519,7 +685,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
 #pragma unroll
                 for (int i = 0; i < kIssues; ++i) {
                     const int row = it.h * p.block_size + ((key0 + gi[i] * 16 + sub[i] * kBoxRows) % p.block_size);
-                    if (has_box[i] && gi[i] < ngroups)
+                    if (has_box[i] && gi[i] < ngroups && (MODE != kShaped || gi[i] * 16 + sub[i] * kBoxRows >= skip))
                         tma_load_3d(smem_u32(ring + (size_t)stage * kKvTileBytes) + off[i], tm, smem_u32(&full[stage]),
                                     hf[i] * 64, row, id[i]);
                 }
@@ -597,7 +763,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             int q_requests = 0;   // items whose rows have been requested so far (phases of q_empty)
             int q_item = -1;      // index (k) of the last item whose rows have been requested or need none
             // 1 = requested, 0 = the previous rows are still being read (only when !blocking), -1 = abort
-            auto request_q = [&](const Item &qi, bool blocking) {
+            auto request_q = [&](const ItemT &qi, bool blocking) {
                 if (q_requests > 0) {
                     uint64_t *bar = &ctrl->q_empty[x];
                     const uint32_t par = (q_requests - 1) & 1;
@@ -636,7 +802,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             for (int k = 0; ok; ++k) {
                 const int item = next_item(k, ok);
                 if (!__all_sync(0xffffffffu, ok) || item < 0) break;
-                const Item it = ctrl->sched_desc[k % kSchedSlots];
+                const ItemT it = ctrl->sched_desc[k % kSchedSlots];
                 const int U = it.nhalf[x], my_tiles = it.ntiles[x];
                 if (U > 0 && q_item < k) {
                     if (request_q(it, true) < 0) {
@@ -715,7 +881,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         for (int k = 0; ok; ++k) {
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
-            const Item it = ctrl->sched_desc[k % kSchedSlots];
+            const ItemT it = ctrl->sched_desc[k % kSchedSlots];
 #pragma unroll
             for (int x = 0; x < kQueryTiles; ++x) {
                 const int U = it.nhalf[x];
@@ -730,6 +896,10 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const bool store = tq_idx < it.tq_valid[x] && row < p.tq * p.group;
                 T *dst = static_cast<T *>(p.out) +
                          ((long long)(it.qoff + it.tok0[x] + tq_idx) * p.num_q_heads + (long long)it.h * p.group + hg) * kD;
+                float *piece = nullptr;                          // kPrefix: the row of the piece's record
+                if constexpr (MODE == kPrefix)
+                    piece = p.prefix_o + ((long long)it.row0 + (long long)blockIdx.x * kPrefixRows +
+                                          (x * p.tq + tq_idx) * p.group + hg) * kD;
                 // the accumulator row in groups of 64 columns: both loads of a group in flight, one wait
                 constexpr int kChunks = kD / 32, kGroup = kChunks < 2 ? kChunks : 2;
 #pragma unroll
@@ -743,7 +913,19 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                         tc_fence_before();
                         mbar_arrive(smem_u32(&ctrl->o_free[x]));
                     }
-                    if (store) {
+                    if (MODE == kPrefix) {
+                        if (store) {
+#pragma unroll
+                            for (int cc = 0; cc < kGroup; ++cc)
+#pragma unroll
+                                for (int i = 0; i < 32; i += 8) {
+                                    uint32_t w[8];
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[cc][i + j] * inv);
+                                    st_global_32B(piece + (c0 + cc) * 32 + i, w);
+                                }
+                        }
+                    } else if (store) {
                         // 32 bytes per lane and instruction: a lane's row is contiguous and the lanes of a warp are a
                         // row apart, so every store instruction fills whole 32-byte sectors
 #pragma unroll
@@ -782,22 +964,35 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         for (int k = 0; ok; ++k) {
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
-            const Item it = ctrl->sched_desc[k % kSchedSlots];
+            const ItemT it = ctrl->sched_desc[k % kSchedSlots];
             const int U = it.nhalf[x];
-            const int pos = it.start + it.tok0[x] + tq_idx;      // last visible key of this row
+            const int t0 = item_t0<MODE>(it);
+            // last visible key of this row
+            const int pos = MODE == kPrefix ? it.ctx_end - 1 : it.start + it.tok0[x] + tq_idx;
+            float slope2 = 0.f;                                  // kShaped: slope of this row's head, log2 domain
+            if constexpr (MODE == kShaped)
+                if (p.slopes != nullptr && row < p.tq * p.group) slope2 = __ldg(p.slopes + it.h * p.group + hg) * 1.4426950408889634f;
             float m_run = -INFINITY, l_run = 0.f;
+            // Before a wait for a V tile at an item's first half-step: this group may be ahead of V tiles of the item before
+            // (it never waits for them otherwise), and a parity wait for a ring stage is only sound once the stage's tile
+            // before has landed.  That one is the group's last tile of the item before when the other query tile had one
+            // tile more (it has at most one), else an older one: the group's last PV product tells.
+            auto v_phase_known = [&]() {
+                return c == 0 || wait_or_abort(smem_u32(&ctrl->pv_done[x][(c - 1) & 1]), ((c - 1) >> 1) & 1, abort_flag, p.status);
+            };
 #pragma unroll 1
             for (int u = 0; ok && u < U; ++u) {
                 const int cu = c + u, buf = cu & 1;
                 const int t = u / kHPT, gt = g + t, stage = gt % kStagesV;
-                const int key0 = u * kHalfKeys;
+                const int key0 = t0 * kTK + u * kHalfKeys;
                 // V rows at or past ctx_end were never written (or never loaded): clear them so that P = 0
                 // there cannot meet a NaN.  Both softmax groups do it (idempotent), at the first half-step of the
                 // key tile, before they release its probabilities.
-                if (u % kHPT == 0 && t * kTK + kTK > it.ctx_end) {
+                if (u % kHPT == 0 && (t0 + t) * kTK + kTK > it.ctx_end) {
+                    if (u == 0 && !(ok = v_phase_known())) break;
                     if (!(ok = wait_or_abort(smem_u32(&ctrl->v_full[stage]), (gt / kStagesV) & 1, abort_flag, p.status))) break;
                     uint8_t *v_tile = v_ring + (size_t)stage * kKvTileBytes;
-                    const int first = max(it.ctx_end - t * kTK, 0);
+                    const int first = max(it.ctx_end - (t0 + t) * kTK, 0);
                     constexpr int kPieces = kHalves * 8;           // 16-byte pieces per row
                     const int n16 = (kTK - first) * kPieces;
                     for (int idx = threadIdx.x & 127; idx < n16; idx += 128) {
@@ -817,12 +1012,44 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 for (int cc = 0; cc < 2; ++cc) tmem_ld32(t_sx + buf * kHalfKeys + cc * 32, sc[cc]);
                 tmem_wait_ld();
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 22, u);
-                if (key0 + kHalfKeys - 1 > it.start + it.tok0[x]) {  // only half-steps that reach past the first row's diagonal
+                float bias0 = 0.f;           // kShaped: the distance bias of the half-step's first key
+                if constexpr (MODE == kShaped) {
+                    if (key0 < it.lo || key0 + kHalfKeys > it.ctx_end) {
+                        // keys that were not read: what their scores happen to be must not choose the branch of the cap
+                        // (the result would depend on it in its last bits)
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (key0 + cc * 32 + i < it.lo || key0 + cc * 32 + i >= it.ctx_end) sc[cc][i] = 0.f;
+                    }
+                    bias0 = shape_scores(sc, slope2, key0 - pos, p);
+                }
+                if constexpr (MODE == kPrefix) {
+                    if (key0 + kHalfKeys > it.ctx_end) {             // keys behind the piece
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
+                    }
+                } else if (key0 + kHalfKeys - 1 > it.start + it.tok0[x]) {  // only half-steps that reach past the first row's diagonal
 #pragma unroll
                     for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
+                }
+                if constexpr (MODE == kShaped) {
+                    // and those that begin before the last row's window
+                    if (key0 <= it.start + it.tok0[x] + p.tq - 1 - p.window) {
+                        const int before = pos - p.window;           // last key that is out of this row's window
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (key0 + cc * 32 + i <= before) sc[cc][i] = -INFINITY;
+                    }
                 }
                 // ---- row maximum: four independent chains of three-input max ----
                 float mxa[4];
@@ -833,7 +1060,9 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
 #pragma unroll
                     for (int q4 = 0; q4 < 4; ++q4)
                         mxa[q4] = fmax3(mxa[q4], sc[q4 >> 1][(q4 & 1) * 16 + i], sc[q4 >> 1][(q4 & 1) * 16 + i + 1]);
-                const float m_new = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * p.scale_log2;
+                const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3]));
+                // kShaped: a half-step that a row sees nothing of (or scores of -inf): any finite maximum serves
+                const float m_new = MODE == kShaped ? fmaxf(mx + bias0, -3.0e38f) : mx * p.scale_log2;
                 if (u == 0) {
                     m_run = m_new;                              // key 0 is visible to every row: finite
                 } else {
@@ -868,14 +1097,16 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 // ---- probabilities (masked scores are -inf -> 0), packed in pairs over the first 32 columns of the
                 //      buffer just read ----
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-                const float2 negm2 = make_float2(-m_run, -m_run);
+                const float negm = MODE == kShaped ? bias0 - m_run : -m_run;
+                const float2 negm2 = make_float2(negm, negm);
                 float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
                     uint32_t packed[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float2 xs = __ffma2_rn(make_float2(sc[cc][2 * i], sc[cc][2 * i + 1]), scale2, negm2);
+                        const float2 raw = make_float2(sc[cc][2 * i], sc[cc][2 * i + 1]);
+                        const float2 xs = MODE == kShaped ? __fadd2_rn(raw, negm2) : __ffma2_rn(raw, scale2, negm2);
                         const float2 pr = (kPolyExpEvery > 0 && i % (kPolyExpEvery > 0 ? kPolyExpEvery : 1) == 0)
                                               ? exp2_fma2(xs)
                                               : make_float2(fast_exp2(xs.x), fast_exp2(xs.y));
@@ -887,6 +1118,21 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const float psum = (acc2[0].x + acc2[1].x) + (acc2[0].y + acc2[1].y);
                 l_run += psum;
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 24, u);
+                if constexpr (MODE == kShaped) {
+                    if (u == 0 && it.lo > key0) {                // V rows before the item's window may hold anything: clear them before PV reads them
+                        if (!(ok = v_phase_known())) break;
+                        if (!(ok = wait_or_abort(smem_u32(&ctrl->v_full[stage]), (gt / kStagesV) & 1, abort_flag, p.status))) break;
+                        uint8_t *v_tile = v_ring + (size_t)stage * kKvTileBytes;
+                        constexpr int kPieces = kHalves * 8;
+                        const int n16 = (it.lo - key0) * kPieces;
+                        for (int idx = threadIdx.x & 127; idx < n16; idx += 128) {
+                            const int r = idx / kPieces, piece = idx % kPieces;
+                            *reinterpret_cast<uint4 *>(v_tile + (piece >> 3) * kKvHalfBytes + r * 128 + ((piece & 7) << 4)) =
+                                make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                }
                 tmem_wait_st();
                 tc_fence_before();           // P is in TMEM, S has been read: the MMA warp may go on
                 mbar_arrive(smem_u32(&ctrl->p_ready[x][buf]));
@@ -903,6 +1149,11 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 if (items_handed > 0 &&
                     !(ok = wait_or_abort(smem_u32(&ctrl->o_free[x]), (items_handed - 1) & 1, abort_flag, p.status))) break;
                 ctrl->l_sum[x][row] = l_run;
+                if constexpr (MODE == kPrefix) {
+                    if (tq_idx < it.tq_valid[x] && row < p.tq * p.group)
+                        p.prefix_lse[(long long)it.row0 + (long long)blockIdx.x * kPrefixRows + (x * p.tq + tq_idx) * p.group + hg] =
+                            m_run + log2f(l_run);
+                }
                 mbar_arrive(smem_u32(&ctrl->epi_ready[x]));
                 ++items_handed;
             }
@@ -921,10 +1172,195 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
     }
     // The last CTA to leave puts the two counters back to zero for the next launch on this workspace (every CTA
     // has drawn its last item by now: its producer warp only leaves its loop on an item past the end, or on abort).
-    if (threadIdx.x == 0 && atomicAdd(p.work_counter + 1, 1) == static_cast<int>(gridDim.x) - 1) {
+    if (MODE != kPrefix && threadIdx.x == 0 && atomicAdd(p.work_counter + 1, 1) == static_cast<int>(gridDim.x) - 1) {
         p.work_counter[0] = 0;
         p.work_counter[1] = 0;
     }
+}
+
+// One call of prompt attention, its arguments as the C ABI names them.
+struct PrefillCall {
+    void *out;
+    const void *q, *k_cache, *v_cache;
+    const int32_t *block_tables, *chunk_q_offset_host, *chunk_tokens_host, *chunk_start_host;
+    int64_t num_chunks;
+    float scale;
+    int64_t num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks, cache_block_stride, bt_row_stride;
+    int dtype;
+    void *workspace;
+    size_t workspace_bytes;
+    int flags;
+    void *stream;
+    int32_t *status = nullptr;       // nullptr: the workspace's first word
+    // kShaped
+    float score_cap = 0.f;
+    const float *slopes = nullptr;
+    int64_t window = 0;              // 0: no window
+};
+
+// What a launch needs beside its parameters: tensor maps, the kernel's instance, shared memory.
+struct PrefillLaunch {
+    CUtensorMap q, k, v;
+    void (*kernel)(PrefillParams, CUtensorMap, CUtensorMap, CUtensorMap);
+    size_t smem;
+    int group, tq, box_rows, query_tiles, tile_keys;
+};
+
+template <int MODE>
+int prepare_launch(const PrefillCall &c, int64_t total_tokens, PrefillLaunch &l) {
+    l.group = static_cast<int>(c.num_q_heads / c.num_kv_heads);
+    l.tq = kRows / l.group;
+    {
+        const uint64_t dims[3] = {(uint64_t)c.head_dim, (uint64_t)c.num_q_heads, (uint64_t)total_tokens};
+        const uint64_t strides[2] = {(uint64_t)c.head_dim * 2u, (uint64_t)c.num_q_heads * c.head_dim * 2u};
+        const uint32_t box[3] = {64u, (uint32_t)l.group, (uint32_t)l.tq};
+        const int rc = npd::encode_tiled_3d(&l.q, c.q, c.dtype, dims, strides, box);
+        if (rc != NPD_OK) return rc;
+    }
+    l.box_rows = c.block_size < 16 ? static_cast<int>(c.block_size) : 16;
+    int rc = npd::encode_cache_tensor_map(&l.k, c.k_cache, c.dtype, c.head_dim, c.num_kv_heads * c.block_size, c.num_blocks,
+                                          c.cache_block_stride, l.box_rows);
+    if (rc != NPD_OK) return rc;
+    rc = npd::encode_cache_tensor_map(&l.v, c.v_cache, c.dtype, c.head_dim, c.num_kv_heads * c.block_size, c.num_blocks,
+                                      c.cache_block_stride, l.box_rows);
+    if (rc != NPD_OK) return rc;
+    const size_t halves = static_cast<size_t>(c.head_dim / 64);
+    l.query_tiles = c.head_dim == 256 ? 1 : 2;
+    l.tile_keys = c.head_dim == 256 ? 64 : kKeys;
+    l.smem = 1024 + l.query_tiles * halves * kQHalfBytes + (size_t)(kStagesK + kStagesV) * halves * l.tile_keys * 128 +
+             sizeof(SmemCtrl) + 64;
+    const bool f16 = c.dtype == NPD_DTYPE_F16;
+#define NPD_PICK_B(D_, B_) (f16 ? paged_prefill_kernel<__half, D_, B_, MODE> : paged_prefill_kernel<__nv_bfloat16, D_, B_, MODE>)
+#define NPD_PICK(D_) l.kernel = l.box_rows == 4 ? NPD_PICK_B(D_, 4) : (l.box_rows == 8 ? NPD_PICK_B(D_, 8) : NPD_PICK_B(D_, 16))
+    if (c.head_dim == 64) NPD_PICK(64);
+    else if (c.head_dim == 128) NPD_PICK(128);
+    else NPD_PICK(256);
+#undef NPD_PICK
+#undef NPD_PICK_B
+    NPD_CUDA_TRY(cudaFuncSetAttribute(l.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.smem));
+    return NPD_OK;
+}
+
+inline void fill_geometry(const PrefillCall &c, const PrefillLaunch &l, PrefillParams &p) {
+    p.scale_log2 = c.scale * 1.4426950408889634f;
+    p.num_q_heads = static_cast<int>(c.num_q_heads);
+    p.num_kv_heads = static_cast<int>(c.num_kv_heads);
+    p.group = l.group;
+    p.tq = l.tq;
+    p.block_size = static_cast<int>(c.block_size);
+    p.box_rows = l.box_rows;
+    p.query_tiles = l.query_tiles;
+    p.half_steps_per_tile = l.tile_keys / kHalfKeys;
+    p.max_blocks_per_seq = static_cast<int>(c.max_blocks_per_seq);
+    p.num_blocks = static_cast<int>(c.num_blocks);
+    p.bt_row_stride = c.bt_row_stride;
+}
+
+// tanh(z) = z P(z^2): P by Remez exchange on z^2 in [0, 1], least relative error 5.9e-7.
+inline void fill_shaping(const PrefillCall &c, PrefillParams &p) {
+    static const double fit[6] = {0.999999413602, -0.333290423701, 0.132814338124, -0.051605672318, 0.0167431133877, -0.00306705973621};
+    p.cap_y = c.score_cap > 0.f ? 2.f * c.scale / c.score_cap : 0.f;
+    p.cap_log2 = c.score_cap * 1.4426950408889634f;
+    double f = 0.5 * c.score_cap * 1.4426950408889634;       // z = y / 2
+    for (int k = 0; k < 6; ++k, f *= 0.25) p.cap_poly[k] = static_cast<float>(fit[k] * f);
+    p.slopes = c.slopes;
+    p.window = c.window > 0 && c.window < INT32_MAX ? static_cast<int>(c.window) : INT32_MAX;
+}
+
+template <int MODE>
+int run_prefill(const PrefillCall &c) {
+    NPD_REQUIRE(c.dtype == NPD_DTYPE_F16 || c.dtype == NPD_DTYPE_BF16, NPD_ERR_UNSUPPORTED,
+                "prefill attention supports float16 and bfloat16 only (dtype code %d)", c.dtype);
+    NPD_REQUIRE(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, NPD_ERR_UNSUPPORTED,
+                "prefill attention: head_dim %lld not in {64,128,256}", (long long)c.head_dim);
+    NPD_REQUIRE(c.block_size == 4 || c.block_size == 8 || c.block_size == 16 || c.block_size == 32, NPD_ERR_UNSUPPORTED,
+                "prefill attention: block_size %lld not in {4,8,16,32}", (long long)c.block_size);
+    NPD_REQUIRE(c.num_chunks >= 0 && c.num_q_heads > 0 && c.num_kv_heads > 0 && c.max_blocks_per_seq > 0 && c.num_blocks > 0,
+                NPD_ERR_INVALID_ARG, "prefill attention: non-positive dimension");
+    NPD_REQUIRE(c.num_q_heads % c.num_kv_heads == 0, NPD_ERR_INVALID_ARG,
+                "prefill attention: num_q_heads is not a multiple of num_kv_heads");
+    const int group = static_cast<int>(c.num_q_heads / c.num_kv_heads);
+    NPD_REQUIRE(group <= 128, NPD_ERR_UNSUPPORTED, "prefill attention: more than 128 q heads per kv head");
+    if (c.num_chunks == 0) return NPD_OK;
+    NPD_REQUIRE(c.out && c.q && c.k_cache && c.v_cache && c.block_tables && c.chunk_q_offset_host && c.chunk_tokens_host &&
+                    c.chunk_start_host,
+                NPD_ERR_INVALID_ARG, "prefill attention: NULL pointer");
+    NPD_REQUIRE(c.workspace != nullptr && c.workspace_bytes >= 256, NPD_ERR_WORKSPACE,
+                "prefill attention: workspace of at least 256 bytes needed (status word)");
+    NPD_REQUIRE(npd::aligned16(c.q) && (reinterpret_cast<uintptr_t>(c.out) & 31u) == 0, NPD_ERR_INVALID_ARG,
+                "prefill attention: q must be 16-byte and out 32-byte aligned");
+    NPD_REQUIRE(c.num_blocks < INT32_MAX && c.max_blocks_per_seq * c.block_size < INT32_MAX, NPD_ERR_INVALID_ARG,
+                "prefill attention: dimension exceeds int32");
+
+    int64_t total_tokens = 0;
+    for (int64_t i = 0; i < c.num_chunks; ++i) {
+        NPD_REQUIRE(c.chunk_tokens_host[i] >= 0 && c.chunk_start_host[i] >= 0 && c.chunk_q_offset_host[i] >= 0,
+                    NPD_ERR_INVALID_ARG, "prefill attention: negative chunk field");
+        NPD_REQUIRE((int64_t)c.chunk_start_host[i] + c.chunk_tokens_host[i] <= c.max_blocks_per_seq * c.block_size,
+                    NPD_ERR_INVALID_ARG, "prefill attention: chunk %lld reaches beyond its block table", (long long)i);
+        const int64_t end = (int64_t)c.chunk_q_offset_host[i] + c.chunk_tokens_host[i];
+        if (end > total_tokens) total_tokens = end;
+    }
+    if (total_tokens == 0) return NPD_OK;
+
+    PrefillLaunch l;
+    int rc = prepare_launch<MODE>(c, total_tokens, l);
+    if (rc != NPD_OK) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+    int dev = 0;
+    NPD_CUDA_TRY(cudaGetDevice(&dev));
+    const long long sms = npd::sm_count(dev);
+    const int tq = l.tq, query_tiles = l.query_tiles;
+    for (int64_t c0 = 0; c0 < c.num_chunks; c0 += kMaxChunks) {
+        const int nc = static_cast<int>(c.num_chunks - c0 < kMaxChunks ? c.num_chunks - c0 : kMaxChunks);
+        PrefillParams p;
+        p.out = c.out;
+        p.block_tables = c.block_tables + c0 * c.bt_row_stride;
+        p.status = c.status ? c.status : static_cast<int32_t *>(c.workspace);
+        p.num_chunks = nc;
+        fill_geometry(c, l, p);
+        if (MODE == kShaped) fill_shaping(c, p);
+#ifdef NPD_PREFILL_TRACE
+        p.trace = c.workspace_bytes >= 256 + 11 * 4096 * sizeof(long long)
+                      ? reinterpret_cast<long long *>(static_cast<uint8_t *>(c.workspace) + 256) : nullptr;
+#endif
+        // Pairs of query tiles of the launch, heaviest (most key tiles) first; the kernel hands them out in
+        // this order through an atomic counter.
+        struct Entry { int weight; uint32_t code; };
+        std::vector<Entry> entries;
+        for (int i = 0; i < nc; ++i) {
+            p.chunk_q_offset[i] = c.chunk_q_offset_host[c0 + i];
+            p.chunk_tokens[i] = c.chunk_tokens_host[c0 + i];
+            p.chunk_start[i] = c.chunk_start_host[c0 + i];
+            const int pairs = (p.chunk_tokens[i] + query_tiles * tq - 1) / (query_tiles * tq);
+            NPD_REQUIRE(pairs <= 0xffff, NPD_ERR_INVALID_ARG, "prefill attention: chunk %d is too long", i);
+            for (int pr = 0; pr < pairs; ++pr) {
+                const int last_tok = std::min(p.chunk_tokens[i], (pr + 1) * query_tiles * tq);
+                int weight = (p.chunk_start[i] + last_tok + kKeys - 1) / kKeys;
+                if (MODE == kShaped) {
+                    const int64_t lo = (int64_t)p.chunk_start[i] + pr * query_tiles * tq - p.window + 1;
+                    if (lo > 0) weight -= static_cast<int>(lo / kKeys);
+                }
+                entries.push_back({weight,
+                                   (static_cast<uint32_t>(i) << 16) | static_cast<uint32_t>(pr)});
+            }
+        }
+        std::stable_sort(entries.begin(), entries.end(), [](const Entry &a, const Entry &b) { return a.weight > b.weight; });
+        cudaStream_t launch_stream = st;
+        for (size_t e0 = 0; e0 < entries.size(); e0 += kMaxPairs) {
+            const int ne = static_cast<int>(std::min<size_t>(kMaxPairs, entries.size() - e0));
+            for (int e = 0; e < ne; ++e) p.pair_order[e] = entries[e0 + e].code;
+            p.num_pairs = ne;
+            p.work_counter = reinterpret_cast<int *>(static_cast<uint8_t *>(c.workspace) + 64);   // zero: see the kernel's end
+            const long long items = (long long)ne * c.num_kv_heads;
+            long long grid = items < sms ? items : sms;           // persistent: one CTA per SM
+            const int cta_cap = (c.flags >> 8) & 0xffff;
+            if (cta_cap > 0 && cta_cap < grid) grid = cta_cap;
+            l.kernel<<<static_cast<unsigned>(grid), kThreads, l.smem, launch_stream>>>(p, l.q, l.k, l.v);
+            NPD_CUDA_TRY(cudaGetLastError());
+        }
+    }
+    return NPD_OK;
 }
 
 }  // namespace

@@ -608,6 +608,108 @@ def paged_scored_attention(out, query, key_cache, value_cache, block_tables, seq
 
 
 # ---------------------------------------------------------------------------
+# (2d) decode attention for a batch that shares prefixes
+# ---------------------------------------------------------------------------
+_shared_plans: Dict[tuple, tuple] = {}
+
+
+def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tables, seq_lens, group_offsets, shared_lens,
+                                  scale: float, block_size: int, max_num_blocks_per_seq: int, max_ctas: int = 0) -> None:
+    """:func:`paged_attention_forward` for a batch whose sequences share the first pages of their tables, written in place.
+
+    Group ``g`` is the sequences ``group_offsets[g] <= s < group_offsets[g + 1]`` (int32 ``[groups + 1]`` on the device, ascending);
+    the first ``shared_lens[g]`` tokens (int32 ``[groups]``) of each lie in the same pages: their ``block_tables`` rows agree there.
+    Those pages are read once per group, on the tensor cores, instead of once per sequence.  Sequences outside every group and
+    groups of one are attended to as usual, and so is what ``shared_lens`` reaches beyond the shortest non-empty sequence of the
+    group.  Lengths, offsets and tables are read on the device, so they may change between replays of a captured call; offsets
+    that do not ascend within the batch are reported by :func:`check_status` and share nothing.  ``block_tables`` is int32
+    ``[S, >= max_num_blocks_per_seq]`` with contiguous rows, at most 4096 groups; the other arguments are those of
+    :func:`paged_attention_forward` (the interleaved layouts are not taken).
+    """
+    try:
+        key = (_sig(out, query, key_cache, value_cache, block_tables, seq_lens, group_offsets, shared_lens), block_size,
+               max_num_blocks_per_seq, max_ctas)
+        plan = _shared_plans.get(key)
+    except (AttributeError, TypeError):
+        raise RuntimeError("paged_shared_prefix_attention takes tensors and numbers") from None
+    if plan is None:
+        name = "paged_shared_prefix_attention"
+        dev, S, hq, hkv, d, bs, nb, cstride, max_blk, row_stride = _check_single_token_call(
+            name, out, query, key_cache, value_cache, block_tables, seq_lens, block_size, max_num_blocks_per_seq)
+        for t, what in ((group_offsets, "group_offsets"), (shared_lens, "shared_lens")):
+            _require(t.dtype == torch.int32 and t.device == dev and t.dim() == 1 and (t.numel() < 2 or t.stride(0) == 1),
+                     f"{name}: {what} must be a contiguous int32 vector on the query's device")
+        groups = shared_lens.numel()
+        _require(1 <= groups <= 4096 and group_offsets.numel() == groups + 1,
+                 f"{name}: between 1 and 4096 groups, group_offsets one longer than shared_lens")
+        _require(0 <= int(max_ctas) <= 0xffff, "max_ctas out of range")
+        if S == 0:
+            return
+        need = _C.npd_shared_prefix_workspace_bytes(S, groups, hq, hkv, d, dev.index)
+        plan = (dev.index, need, 256 + 4 * S * hq, int(max_ctas) << 8,
+                (S, groups, hq, hkv, d, bs, max_blk, nb, cstride, row_stride, _DTYPE_CODE[query.dtype]))
+        _remember(_shared_plans, key, plan)
+    dev_index, need, cleared, flags, args = plan
+    handle = _raw_stream(dev_index)
+    ws = _scratch_for(dev_index, handle, need, min(cleared, need))
+    _call(dev_index, _C.npd_paged_shared_prefix_attention, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+          block_tables.data_ptr(), seq_lens.data_ptr(), group_offsets.data_ptr(), shared_lens.data_ptr(), float(scale), *args,
+          ws.data_ptr(), ws.numel(), _status_ptr(dev_index), flags, handle)
+
+
+# ---------------------------------------------------------------------------
+# (3b) chunked-prefill attention with shaped scores
+# ---------------------------------------------------------------------------
+def paged_scored_prefill_attention(out, query, key_cache, value_cache, block_tables, chunk_q_offsets: Sequence[int],
+                                   chunk_tokens: Sequence[int], chunk_starts: Sequence[int], scale: float, block_size: int,
+                                   max_num_blocks_per_seq: int, score_cap: float = 0.0, distance_slopes=None, window: int = 0,
+                                   max_ctas: int = 0) -> None:
+    """:func:`paged_prefill_attention` with the scores shaped before the softmax, written in place.
+
+    The shaping is that of :func:`paged_scored_attention`: a query at position ``i`` sees the keys ``i - window < j <= i`` (all up to
+    ``i`` with ``window == 0``), its distance to key ``j`` is ``i - j``.  Pages wholly before the window of a chunk's first query are
+    not read and their table entries may be stale.  The other arguments are those of :func:`paged_prefill_attention`.
+    """
+    name = "paged_scored_prefill_attention"
+    try:
+        _require(query.is_cuda and query.dim() == 3, f"{name}: query must be a CUDA tensor [tokens, num_heads, head_size]")
+        _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2, f"{name}: block_tables must be int32 [chunks, max_blk]")
+        dev = query.device
+        total, hq, d = query.shape
+        nchunks = len(chunk_tokens)
+        _require(len(chunk_q_offsets) == nchunks and len(chunk_starts) == nchunks and block_tables.size(0) == nchunks,
+                 f"{name}: one offset, token count, start position and table row per chunk")
+        _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and query.is_contiguous() and out.is_contiguous(),
+                 f"{name}: out must match query in shape, dtype and device; both contiguous")
+        _require(query.dtype in (torch.float16, torch.bfloat16), f"{name}: unsupported dtype {query.dtype}")
+        nb, hkv, bs, cd, cstride = _cache_geometry(key_cache, "key_cache")
+        _require(_cache_geometry(value_cache, "value_cache") == (nb, hkv, bs, cd, cstride), "cache layouts differ")
+        _require(cd == d and int(block_size) == bs and key_cache.dtype == query.dtype == value_cache.dtype, f"{name}: cache does not match query")
+        _require(all(t.device == dev for t in (key_cache, value_cache, block_tables)), f"{name}: all tensors must be on the query's device")
+        _require(hq % hkv == 0, "num_heads must be a multiple of num_kv_heads")
+        _require(block_tables.stride(1) == 1 or block_tables.size(1) == 1, "block_tables rows must be contiguous")
+        max_blk = int(max_num_blocks_per_seq)
+        _require(1 <= max_blk <= block_tables.size(1), "max_num_blocks_per_seq out of range")
+        _require(0 <= int(max_ctas) <= 0xffff, "max_ctas out of range")
+        _score_shape(name, score_cap, distance_slopes, window, hq, dev)
+    except (AttributeError, TypeError):
+        raise RuntimeError(f"{name} takes tensors, lists of whole numbers and numbers") from None
+    for off, n, start in zip(chunk_q_offsets, chunk_tokens, chunk_starts):
+        _require(n >= 0 and off >= 0 and off + n <= total and start >= 0, f"{name}: chunk outside the query tensor")
+        _require(start + n <= max_blk * bs, f"{name}: chunk reaches beyond its block table")
+    if nchunks == 0 or total == 0:
+        return
+    arr = ctypes.c_int32 * nchunks
+    handle = _raw_stream(dev.index)
+    need = _C.npd_prefill_workspace_bytes(total, hq, hkv, d, dev.index)
+    ws = _scratch_for(dev.index, handle, need, 256)
+    _call(dev.index, _C.npd_paged_scored_prefill_attention, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+          block_tables.data_ptr(), arr(*chunk_q_offsets), arr(*chunk_tokens), arr(*chunk_starts), nchunks, float(scale), float(score_cap),
+          None if distance_slopes is None else distance_slopes.data_ptr(), int(window), hq, hkv, d, bs, max_blk, nb, cstride,
+          block_tables.stride(0), _DTYPE_CODE[query.dtype], ws.data_ptr(), ws.numel(), _status_ptr(dev.index), int(max_ctas) << 8, handle)
+
+
+# ---------------------------------------------------------------------------
 # (4) KV page migration
 # ---------------------------------------------------------------------------
 def _pool_geometry(pool: torch.Tensor, name: str):

@@ -10,4 +10,6 @@ from nanopd_b200.paged_kernels import (  # noqa: F401
     paged_prefill_attention,
     paged_qk_norm_rope_store,
     paged_scored_attention,
+    paged_scored_prefill_attention,
+    paged_shared_prefix_attention,
 )

@@ -292,3 +292,33 @@ def test_head_dim_96_is_refused(kernels):
     with pytest.raises(RuntimeError, match="head_dim"):
         kernels.paged_prefill_attention(torch.zeros_like(q), q, kc, kc.clone(), torch.zeros(1, 1, dtype=torch.int32, device=DEV),
                                         [0], [4], [0], 1.0, 16, 1)
+
+
+@pytest.mark.parametrize("repeat", range(3))
+def test_short_items_behind_pairs_of_unequal_reach(kernels, repeat):
+    """One CTA works through pairs whose second query tile needs a key tile more than the first, each followed by an item
+    of one partial key tile: its unwritten V rows (NaN here) must be cleared in the tile it reads, not in an earlier one."""
+    hq, hkv, d, block = 32, 8, 128, 16
+    chunks = [(96, 64)] * 20 + [(0, 21)] * 20
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(repeat)
+    need = [-(-(s + n) // block) for s, n in chunks]
+    kc, vc = (torch.full((sum(need), hkv, block, d), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    bt = torch.zeros(len(chunks), max(need), dtype=torch.int32, device=DEV)
+    at, offs = 0, []
+    for i, (s, n) in enumerate(chunks):
+        bt[i, :need[i]] = torch.arange(at, at + need[i], device=DEV)
+        for c in (kc, vc):
+            rows = torch.randn(s + n, hkv, d, generator=gen, device=DEV).to(c.dtype)
+            for j in range(need[i]):
+                part = rows[j * block:(j + 1) * block]
+                c[at + j, :, :part.size(0)] = part.transpose(0, 1)
+        at += need[i]
+        offs.append(sum(m for _, m in chunks[:i]))
+    q = torch.randn(sum(n for _, n in chunks), hq, d, generator=gen, device=DEV).to(torch.bfloat16)
+    out, alone = torch.empty_like(q), torch.empty_like(q)
+    args = (kc, vc, bt, offs, [n for _, n in chunks], [s for s, _ in chunks], d ** -0.5, block, bt.size(1))
+    kernels.paged_prefill_attention(out, q, *args, max_ctas=1)
+    kernels.paged_prefill_attention(alone, q, *args)
+    torch.cuda.synchronize()
+    assert torch.isfinite(out).all() and torch.equal(out, alone)
