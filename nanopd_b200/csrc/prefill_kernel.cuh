@@ -39,6 +39,7 @@
 // Algorithmic flops per chunk: 4*Hq*D*(n*start + n(n+1)/2)  (causal; masked work not counted).
 #pragma once
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "npd_common.cuh"
@@ -83,11 +84,13 @@ constexpr long long kWaitCycles = 4000000000LL;
 
 // What the kernel computes (template parameter MODE):
 //   kCausal  prompt chunks, plain causal attention
-//   kShaped  prompt chunks with capped scores, a distance bias and a sliding window (each optional)
+//   kShaped  prompt chunks with a distance bias and a sliding window (each optional)
+//   kCapped  the same with scores capped by a tanh
 //   kPrefix  a decode batch's queries over the shared prefix of their group: every key of a piece of the prefix is visible
 //            to every row, and the rows leave as fp32 with their log2 sums, to be joined with the rest of each sequence.
 //            A CTA takes an equal run of (group, query tiles, kv head, key tile) units, cut where items end.
-enum : int { kCausal = 0, kShaped = 1, kPrefix = 2 };
+enum : int { kCausal = 0, kShaped = 1, kPrefix = 2, kCapped = 3 };
+__host__ __device__ constexpr bool shapes(int mode) { return mode == kShaped || mode == kCapped; }
 
 struct PrefillParams {
     void *out;
@@ -107,11 +110,13 @@ struct PrefillParams {
     int chunk_q_offset[kMaxChunks];
     int chunk_tokens[kMaxChunks];
     int chunk_start[kMaxChunks];
-    // kShaped; the score in the log2 domain is y * R(y^2) with y = 2 scale/cap * (q . k) below |y| = 2 (R: cap_poly), and
-    // cap_log2 - 2 cap_log2 / (1 + e^y) elsewhere (y = 2z: tanh z = 1 - 2 / (1 + e^2z))
-    float cap_y;                      // 2 * scale / cap; 0 = scores are not capped
+    // kCapped: a capped score in the log2 domain is x Q(x^2), x = q . k, for |x| < cap_reach (Q: cap_poly), and
+    // cap_log2 - 2 cap_log2 / (1 + 2^(cap_in x)) elsewhere (tanh z = 1 - 2 / (1 + e^2z))
+    float cap_in;                     // 2 log2(e) * scale / cap
     float cap_log2;                   // cap * log2(e)
-    float cap_poly[6];
+    float cap_reach;
+    float cap_poly[4];
+    // kShaped, kCapped
     const float *slopes;              // [num_q_heads] or nullptr
     int window;                       // keys visible behind a query, its own included; INT32_MAX = all
     // kPrefix
@@ -243,66 +248,61 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Maximum / minimum of a row's 64 scores: four independent chains of three-input operations.
+__device__ __forceinline__ float row_max(const float (&sc)[2][32]) {
+    float m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) m[q] = fmaxf(sc[q >> 1][(q & 1) * 16], sc[q >> 1][(q & 1) * 16 + 1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m[q] = fmax3(m[q], sc[q >> 1][(q & 1) * 16 + i], sc[q >> 1][(q & 1) * 16 + i + 1]);
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+__device__ __forceinline__ float row_min(const float (&sc)[2][32]) {
+    float m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) m[q] = fminf(sc[q >> 1][(q & 1) * 16], sc[q >> 1][(q & 1) * 16 + 1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m[q] = fmin3(m[q], sc[q >> 1][(q & 1) * 16 + i], sc[q >> 1][(q & 1) * 16 + i + 1]);
+    return fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
+}
 
-// Shapes the 64 raw scores of a row's half-step in place (cap, distance bias), into the log2 domain; `rel` is the first
-// key's position relative to the query's.  Returns what is still to be added to each of them, the bias of the first key.
-// The cap: tanh(z) = z P(z^2) on |z| < 1, P of degree 5 fitted by Remez exchange for the least relative error (6e-7);
-// y = 2z carries the test for it: an exponent of 128 or more, that is |y| >= 2, an infinity or a NaN, sets bit 30, and one
-// OR over the row finds it.  Scores as large as the cap are rare (a cap tames the rare ones), so the warp's test almost
-// never takes the second branch, an exponential and a reciprocal per score: three special-function results a score would
-// bound the kernel (8192 scores per query tile and half-step at 16 a clock are 1536 clocks; the two products take 512).
+// Shapes the 64 raw scores of a row's half-step in place, into the log2 domain, whatever their size: cap and distance bias.
+// `rel` is the first key's position relative to the query's.  Returns what is still to be added to each score, the bias of
+// the first key.
+template <bool kCap>
 __device__ __forceinline__ float shape_scores(float (&sc)[2][32], float slope2, int rel, const PrefillParams &p) {
-    if (p.cap_y != 0.f) {
-        const float2 c2 = make_float2(p.cap_y, p.cap_y);
-        uint32_t bits = 0;
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float2 y = __fmul2_rn(make_float2(sc[cc][i], sc[cc][i + 1]), c2);
-                sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
-                bits |= __float_as_uint(y.x) | __float_as_uint(y.y);
-            }
-        if (__any_sync(0xffffffffu, (bits & 0x40000000u) != 0)) {
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    sc[cc][i] = p.cap_log2 - __fdividef(2.f * p.cap_log2, 1.f + fast_exp2(sc[cc][i] * 1.4426950408889634f));
-        } else {
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 y = make_float2(sc[cc][i], sc[cc][i + 1]), w = __fmul2_rn(y, y);
-                    float2 q = make_float2(p.cap_poly[5], p.cap_poly[5]);
-#pragma unroll
-                    for (int k = 4; k >= 0; --k) q = __ffma2_rn(q, w, make_float2(p.cap_poly[k], p.cap_poly[k]));
-                    q = __fmul2_rn(q, y);
-                    sc[cc][i] = q.x, sc[cc][i + 1] = q.y;
-                }
-        }
-    } else {
-        const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float2 y = __fmul2_rn(make_float2(sc[cc][i], sc[cc][i + 1]), c2);
-                sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
-            }
-    }
-    if (p.slopes == nullptr) return 0.f;
-    const float2 s2 = make_float2(slope2, slope2);
+    const float2 c2 = make_float2(p.scale_log2, p.scale_log2), s2 = make_float2(slope2, slope2);
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            const float2 y = __ffma2_rn(make_float2(static_cast<float>(cc * 32 + i), static_cast<float>(cc * 32 + i + 1)), s2,
-                                        make_float2(sc[cc][i], sc[cc][i + 1]));
+            float2 y = make_float2(sc[cc][i], sc[cc][i + 1]);
+            if (kCap) {
+                y.x = p.cap_log2 - __fdividef(2.f * p.cap_log2, 1.f + fast_exp2(y.x * p.cap_in));
+                y.y = p.cap_log2 - __fdividef(2.f * p.cap_log2, 1.f + fast_exp2(y.y * p.cap_in));
+            } else {
+                y = __fmul2_rn(y, c2);
+            }
+            y = __ffma2_rn(make_float2(static_cast<float>(cc * 32 + i), static_cast<float>(cc * 32 + i + 1)), s2, y);
             sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
         }
     return slope2 * static_cast<float>(rel);
+}
+// Q of the cap for a pair of squares.
+__device__ __forceinline__ float2 cap_factor2(float2 w, const PrefillParams &p) {
+    float2 q = make_float2(p.cap_poly[3], p.cap_poly[3]);
+#pragma unroll
+    for (int k = 2; k >= 0; --k) q = __ffma2_rn(q, w, make_float2(p.cap_poly[k], p.cap_poly[k]));
+    return q;
 }
 
 // Shared-memory matrix descriptors (version 1, 128-byte swizzle, 8-row groups 1024 B apart).
@@ -421,7 +421,7 @@ __device__ __forceinline__ typename ItemOf<MODE>::type decode_item(const Prefill
     it.qoff = p.chunk_q_offset[c];
     it.ctx_end = it.start + n_tok;                              // keys written so far for this sequence
     int skipped = 0;                                            // half-steps in front of the first tile walked
-    if constexpr (MODE == kShaped) {
+    if constexpr (shapes(MODE)) {
         const long long lo = (long long)it.start + p.query_tiles * pair * p.tq - p.window + 1;   // of the item's first query
         it.lo = lo > 0 ? static_cast<int>(lo) : 0;
         it.t0 = it.lo / (kHalfKeys * p.half_steps_per_tile);
@@ -645,7 +645,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const int key = (t0 + t) * kTK + gi[i] * 16 + sub[i] * kBoxRows;
                 int id = 0;
                 bool wanted = has_box[i] && t < it.n_kv && key < it.ctx_end;
-                if constexpr (MODE == kShaped) wanted = wanted && key + kBoxRows > it.lo;
+                if constexpr (shapes(MODE)) wanted = wanted && key + kBoxRows > it.lo;
                 if (wanted) {
                     id = __ldg(table + key / p.block_size);
                     if (id < 0 || id >= p.num_blocks) {
@@ -671,7 +671,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 for (int g2 = 0; g2 < kTK / 16; ++g2) ngroups += (key0 + g2 * 16 < it.ctx_end) ? 1 : 0;
                 // boxes wholly before the window are not read either: their pages may have been given away
                 int skip = 0;                                   // keys of the tile in front of the first box read
-                if constexpr (MODE == kShaped) skip = max(0, it.lo - key0) / kBoxRows * kBoxRows;
+                if constexpr (shapes(MODE)) skip = max(0, it.lo - key0) / kBoxRows * kBoxRows;
                 const uint32_t bytes = static_cast<uint32_t>((ngroups * 16 - skip) * kHalves * 128);
                 // the stage is free once the MMAs that read the tile `stages` tiles back are done: the score MMAs
                 // for a K tile, the PV MMAs for a V tile
@@ -685,7 +685,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
 #pragma unroll
                 for (int i = 0; i < kIssues; ++i) {
                     const int row = it.h * p.block_size + ((key0 + gi[i] * 16 + sub[i] * kBoxRows) % p.block_size);
-                    if (has_box[i] && gi[i] < ngroups && (MODE != kShaped || gi[i] * 16 + sub[i] * kBoxRows >= skip))
+                    if (has_box[i] && gi[i] < ngroups && (!shapes(MODE) || gi[i] * 16 + sub[i] * kBoxRows >= skip))
                         tma_load_3d(smem_u32(ring + (size_t)stage * kKvTileBytes) + off[i], tm, smem_u32(&full[stage]),
                                     hf[i] * 64, row, id[i]);
                 }
@@ -970,7 +970,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             // last visible key of this row
             const int pos = MODE == kPrefix ? it.ctx_end - 1 : it.start + it.tok0[x] + tq_idx;
             float slope2 = 0.f;                                  // kShaped: slope of this row's head, log2 domain
-            if constexpr (MODE == kShaped)
+            if constexpr (shapes(MODE))
                 if (p.slopes != nullptr && row < p.tq * p.group) slope2 = __ldg(p.slopes + it.h * p.group + hg) * 1.4426950408889634f;
             float m_run = -INFINITY, l_run = 0.f;
             // Before a wait for a V tile at an item's first half-step: this group may be ahead of V tiles of the item before
@@ -1012,57 +1012,44 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 for (int cc = 0; cc < 2; ++cc) tmem_ld32(t_sx + buf * kHalfKeys + cc * 32, sc[cc]);
                 tmem_wait_ld();
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 22, u);
-                float bias0 = 0.f;           // kShaped: the distance bias of the half-step's first key
-                if constexpr (MODE == kShaped) {
-                    if (key0 < it.lo || key0 + kHalfKeys > it.ctx_end) {
-                        // keys that were not read: what their scores happen to be must not choose the branch of the cap
-                        // (the result would depend on it in its last bits)
-#pragma unroll
-                        for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (key0 + cc * 32 + i < it.lo || key0 + cc * 32 + i >= it.ctx_end) sc[cc][i] = 0.f;
+                const int first_pos = it.start + it.tok0[x];       // of the tile's first row
+                const bool diagonal = key0 + kHalfKeys - 1 > first_pos;      // reaches past the first row's diagonal
+                float m_new, bias0 = 0.f;    // bias0: the distance bias of the half-step's first key
+                bool direct = false;         // kCapped: the scores are still raw, their cap is a polynomial
+                if constexpr (shapes(MODE)) {
+                    const bool behind = key0 <= first_pos + p.tq - 1 - p.window;     // begins before the last row's window
+                    if (MODE == kCapped && !diagonal && !behind && p.slopes == nullptr) {
+                        // tanh grows with its argument: the largest capped score is that of the largest raw one
+                        const float mx = row_max(sc);
+                        direct = !__any_sync(0xffffffffu, fmaxf(mx, -row_min(sc)) >= p.cap_reach);
+                        if (direct) m_new = mx * cap_factor2(make_float2(mx * mx, 0.f), p).x;
                     }
-                    bias0 = shape_scores(sc, slope2, key0 - pos, p);
-                }
-                if constexpr (MODE == kPrefix) {
-                    if (key0 + kHalfKeys > it.ctx_end) {             // keys behind the piece
+                    if (!direct) {
+                        if (MODE == kCapped || p.slopes != nullptr) bias0 = shape_scores<MODE == kCapped>(sc, slope2, key0 - pos, p);
+                        if (diagonal || behind) {
+                            const int before = pos - p.window;           // last key that is out of this row's window
+#pragma unroll
+                            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const int key = key0 + cc * 32 + i;
+                                    if (key > pos || key <= before) sc[cc][i] = -INFINITY;
+                                }
+                        }
+                        // a half-step that a row sees nothing of (or scores of -inf): any finite maximum serves
+                        m_new = fmaxf(row_max(sc) * (MODE == kShaped && p.slopes == nullptr ? p.scale_log2 : 1.f) + bias0, -3.0e38f);
+                    }
+                } else {
+                    // kPrefix: only keys behind the piece are masked
+                    if (MODE == kPrefix ? key0 + kHalfKeys > it.ctx_end : diagonal) {
 #pragma unroll
                         for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
                                 if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
                     }
-                } else if (key0 + kHalfKeys - 1 > it.start + it.tok0[x]) {  // only half-steps that reach past the first row's diagonal
-#pragma unroll
-                    for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
+                    m_new = row_max(sc) * p.scale_log2;
                 }
-                if constexpr (MODE == kShaped) {
-                    // and those that begin before the last row's window
-                    if (key0 <= it.start + it.tok0[x] + p.tq - 1 - p.window) {
-                        const int before = pos - p.window;           // last key that is out of this row's window
-#pragma unroll
-                        for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (key0 + cc * 32 + i <= before) sc[cc][i] = -INFINITY;
-                    }
-                }
-                // ---- row maximum: four independent chains of three-input max ----
-                float mxa[4];
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) mxa[q4] = fmaxf(sc[q4 >> 1][(q4 & 1) * 16], sc[q4 >> 1][(q4 & 1) * 16 + 1]);
-#pragma unroll
-                for (int i = 2; i < 16; i += 2)
-#pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4)
-                        mxa[q4] = fmax3(mxa[q4], sc[q4 >> 1][(q4 & 1) * 16 + i], sc[q4 >> 1][(q4 & 1) * 16 + i + 1]);
-                const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3]));
-                // kShaped: a half-step that a row sees nothing of (or scores of -inf): any finite maximum serves
-                const float m_new = MODE == kShaped ? fmaxf(mx + bias0, -3.0e38f) : mx * p.scale_log2;
                 if (u == 0) {
                     m_run = m_new;                              // key 0 is visible to every row: finite
                 } else {
@@ -1096,9 +1083,20 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 23, u);
                 // ---- probabilities (masked scores are -inf -> 0), packed in pairs over the first 32 columns of the
                 //      buffer just read ----
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-                const float negm = MODE == kShaped ? bias0 - m_run : -m_run;
+                const float scale1 = MODE == kShaped && p.slopes != nullptr ? 1.f : p.scale_log2;
+                const float2 scale2 = make_float2(scale1, scale1);
+                const float negm = shapes(MODE) ? bias0 - m_run : -m_run;
                 const float2 negm2 = make_float2(negm, negm);
+                if constexpr (MODE == kCapped) {
+#pragma unroll
+                    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float2 y = make_float2(sc[cc][i], sc[cc][i + 1]);
+                            y = direct ? __ffma2_rn(cap_factor2(__fmul2_rn(y, y), p), y, negm2) : __fadd2_rn(y, negm2);
+                            sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
+                        }
+                }
                 float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
@@ -1106,7 +1104,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float2 raw = make_float2(sc[cc][2 * i], sc[cc][2 * i + 1]);
-                        const float2 xs = MODE == kShaped ? __fadd2_rn(raw, negm2) : __ffma2_rn(raw, scale2, negm2);
+                        const float2 xs = MODE == kCapped ? raw : __ffma2_rn(raw, scale2, negm2);
                         const float2 pr = (kPolyExpEvery > 0 && i % (kPolyExpEvery > 0 ? kPolyExpEvery : 1) == 0)
                                               ? exp2_fma2(xs)
                                               : make_float2(fast_exp2(xs.x), fast_exp2(xs.y));
@@ -1118,7 +1116,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const float psum = (acc2[0].x + acc2[1].x) + (acc2[0].y + acc2[1].y);
                 l_run += psum;
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 24, u);
-                if constexpr (MODE == kShaped) {
+                if constexpr (shapes(MODE)) {
                     if (u == 0 && it.lo > key0) {                // V rows before the item's window may hold anything: clear them before PV reads them
                         if (!(ok = v_phase_known())) break;
                         if (!(ok = wait_or_abort(smem_u32(&ctrl->v_full[stage]), (gt / kStagesV) & 1, abort_flag, p.status))) break;
@@ -1256,13 +1254,22 @@ inline void fill_geometry(const PrefillCall &c, const PrefillLaunch &l, PrefillP
     p.bt_row_stride = c.bt_row_stride;
 }
 
-// tanh(z) = z P(z^2): P by Remez exchange on z^2 in [0, 1], least relative error 5.9e-7.
+// The cap as a polynomial: tanh(z) = z P(z^2) for |z| < 0.6, P of degree 3 fitted by Remez exchange for the least relative
+// error, 2.1e-6 (at the largest score it serves, cap * tanh(0.6), that is 1.1e-6 cap).  With x = q . k and z = x scale / cap,
+// cap log2(e) tanh(z) = x Q(x^2).  Four multiply-adds a score; an exponential and a reciprocal beside the softmax's own
+// exponential, as for the scores beyond, would bound the kernel by its special-function unit: 16384 scores of a half-step of
+// both query tiles at 16 a clock are 1024 clocks for each, the tensor cores need 1024 for the products.  Scores beyond 0.6
+// cap are what a cap is there for, but they are rare.
 inline void fill_shaping(const PrefillCall &c, PrefillParams &p) {
-    static const double fit[6] = {0.999999413602, -0.333290423701, 0.132814338124, -0.051605672318, 0.0167431133877, -0.00306705973621};
-    p.cap_y = c.score_cap > 0.f ? 2.f * c.scale / c.score_cap : 0.f;
+    static const double fit[4] = {0.999997851257, -0.333140392051, 0.130578560594, -0.0409294240958};
+    const double per = c.score_cap > 0.f ? (double)c.scale / c.score_cap : 0.0;
+    p.cap_in = static_cast<float>(2.0 * 1.4426950408889634 * per);
     p.cap_log2 = c.score_cap * 1.4426950408889634f;
-    double f = 0.5 * c.score_cap * 1.4426950408889634;       // z = y / 2
-    for (int k = 0; k < 6; ++k, f *= 0.25) p.cap_poly[k] = static_cast<float>(fit[k] * f);
+    // the coefficients fall by per^2 each: far outside the usual range they would leave fp32's, and no score takes them
+    const bool usual = fabs(per) > 1e-4 && fabs(per) < 1e4 && c.score_cap > 1e-6f && c.score_cap < 1e6f;
+    p.cap_reach = usual ? static_cast<float>(0.6 / fabs(per)) : 0.f;
+    double f = c.score_cap * 1.4426950408889634 * per;
+    for (int k = 0; k < 4; ++k, f *= per * per) p.cap_poly[k] = usual ? static_cast<float>(fit[k] * f) : 0.f;
     p.slopes = c.slopes;
     p.window = c.window > 0 && c.window < INT32_MAX ? static_cast<int>(c.window) : INT32_MAX;
 }
@@ -1319,7 +1326,7 @@ int run_prefill(const PrefillCall &c) {
         p.status = c.status ? c.status : static_cast<int32_t *>(c.workspace);
         p.num_chunks = nc;
         fill_geometry(c, l, p);
-        if (MODE == kShaped) fill_shaping(c, p);
+        if (shapes(MODE)) fill_shaping(c, p);
 #ifdef NPD_PREFILL_TRACE
         p.trace = c.workspace_bytes >= 256 + 11 * 4096 * sizeof(long long)
                       ? reinterpret_cast<long long *>(static_cast<uint8_t *>(c.workspace) + 256) : nullptr;
@@ -1337,7 +1344,7 @@ int run_prefill(const PrefillCall &c) {
             for (int pr = 0; pr < pairs; ++pr) {
                 const int last_tok = std::min(p.chunk_tokens[i], (pr + 1) * query_tiles * tq);
                 int weight = (p.chunk_start[i] + last_tok + kKeys - 1) / kKeys;
-                if (MODE == kShaped) {
+                if (shapes(MODE)) {
                     const int64_t lo = (int64_t)p.chunk_start[i] + pr * query_tiles * tq - p.window + 1;
                     if (lo > 0) weight -= static_cast<int>(lo / kKeys);
                 }

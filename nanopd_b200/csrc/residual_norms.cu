@@ -81,8 +81,7 @@ template <> struct Vec8<__nv_bfloat16> : Vec8Half<__nv_bfloat16, __nv_bfloat162>
 
 constexpr int kMaxThreads = 512;
 
-// Sum over the warps of one row; every thread of the CTA takes part.  `buf`: one float per warp of the CTA, not read
-// again before the next barrier (the two sums of a row use two buffers).
+// Sum over the warps of one row; every thread of the CTA takes part.  `buf`: one float per warp of the CTA.
 __device__ __forceinline__ float row_sum(float v, int warps_per_row, float *buf) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -95,102 +94,121 @@ __device__ __forceinline__ float row_sum(float v, int warps_per_row, float *buf)
     return s;
 }
 
+// A CTA takes every gridDim-th set of rows; the loads of its next set are issued before it works on this one, and the
+// weights stay in registers (16 bits each).
 template <typename T, int kVecs>
 __global__ void __launch_bounds__(kMaxThreads) residual_norms_kernel(const NormParams p) {
-    __shared__ float sums[2][kMaxThreads / 32];
-    const int row_threads = p.warps_per_row * 32;
+    // two buffers per sum: a fast warp may be a row ahead of a slow one that still reads
+    __shared__ float sums[2][2][kMaxThreads / 32];
+    const int row_threads = p.warps_per_row * 32, rows_per_cta = blockDim.x / row_threads;
     const int sub = threadIdx.x / row_threads, t = threadIdx.x - sub * row_threads;
-    const long long row = (long long)blockIdx.x * (blockDim.x / row_threads) + sub;
-    const bool live = row < p.num_rows;
-    const T *x = static_cast<const T *>(p.x) + row * p.x_stride, *res = static_cast<const T *>(p.residual) + row * p.residual_stride;
-    const T *gate = static_cast<const T *>(p.gate) + row * p.gate_stride;
+    const bool post = p.post_weight != nullptr, gated = p.gate != nullptr, gate_per_row = gated && p.gate_stride != 0;
 
-    // plain loads of x and residual: the outputs may be the same rows
-    Vec8<T> xv[kVecs], rv[kVecs];
+    Vec8<T> wv[kVecs], pv[kVecs], gv[kVecs], xv[kVecs], rv[kVecs];
+    auto load_rows = [&](long long row) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int v = t + i * row_threads;
+            if (row >= p.num_rows || v >= p.vecs) continue;
+            // plain loads: the outputs may be the same rows
+            xv[i].load(static_cast<const T *>(p.x) + row * p.x_stride + v * 8);
+            rv[i].load(static_cast<const T *>(p.residual) + row * p.residual_stride + v * 8);
+            if (gate_per_row) gv[i].load(static_cast<const T *>(p.gate) + row * p.gate_stride + v * 8);
+        }
+    };
+    long long row = (long long)blockIdx.x * rows_per_cta + sub;
+    load_rows(row);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
         const int v = t + i * row_threads;
-        if (live && v < p.vecs) {
-            xv[i].load(x + v * 8);
-            rv[i].load(res + v * 8);
-        }
+        if (v >= p.vecs) continue;
+        wv[i].load(static_cast<const T *>(p.weight) + v * 8);
+        if (post) pv[i].load(static_cast<const T *>(p.post_weight) + v * 8);
+        if (gated && !gate_per_row) gv[i].load(static_cast<const T *>(p.gate) + v * 8);
     }
-    float inv = p.residual_scale;
-    if (p.post_weight != nullptr) {
+    int turn = 0;
+    for (long long row0 = (long long)blockIdx.x * rows_per_cta; row0 < p.num_rows; row0 += (long long)gridDim.x * rows_per_cta) {
+        const long long row = row0 + sub;
+        float y[kVecs][8], r[kVecs][8];
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-            if (!live || t + i * row_threads >= p.vecs) continue;
-            float f[8];
-            xv[i].unpack(f);
+            if (row >= p.num_rows || t + i * row_threads >= p.vecs) continue;
+            xv[i].unpack(y[i]);
+            rv[i].unpack(r[i]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+            for (int e = 0; e < 8; ++e) ss += y[i][e] * y[i][e];
+            if (gated) {
+                float g[8];
+                gv[i].unpack(g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[i][e] *= g[e];
+            }
         }
-        inv *= rsqrtf(row_sum(ss, p.warps_per_row, sums[0]) * p.inv_hidden + p.eps);
+        load_rows(row + (long long)gridDim.x * rows_per_cta);
+        float inv = p.residual_scale;
+        if (post) inv *= rsqrtf(row_sum(ss, p.warps_per_row, sums[turn][0]) * p.inv_hidden + p.eps);
+        ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int v = t + i * row_threads;
+            if (row >= p.num_rows || v >= p.vecs) continue;
+            if (post) {
+                float w[8];
+                pv[i].unpack(w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[i][e] *= w[e] + p.offset;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                r[i][e] += y[i][e] * inv;
+                ss += r[i][e] * r[i][e];
+            }
+            Vec8<T> o;
+            o.pack(r[i]);
+            o.store(static_cast<T *>(p.residual_out) + row * p.residual_out_stride + v * 8);
+        }
+        const float inv_r = rsqrtf(row_sum(ss, p.warps_per_row, sums[turn][1]) * p.inv_hidden + p.eps);
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int v = t + i * row_threads;
+            if (row >= p.num_rows || v >= p.vecs) continue;
+            float w[8];
+            wv[i].unpack(w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[i][e] *= inv_r * (w[e] + p.offset);
+            Vec8<T> o;
+            o.pack(r[i]);
+            o.store(static_cast<T *>(p.out) + row * p.out_stride + v * 8);
+        }
+        turn ^= 1;
     }
-    float r[kVecs][8];
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int v = t + i * row_threads;
-        if (!live || v >= p.vecs) continue;
-        float f[8];
-        xv[i].unpack(f);
-        rv[i].unpack(r[i]);
-        if (p.post_weight != nullptr) {
-            Vec8<T> w;
-            float wf[8];
-            w.load(static_cast<const T *>(p.post_weight) + v * 8);
-            w.unpack(wf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= wf[e] + p.offset;
-        }
-        if (p.gate != nullptr) {
-            Vec8<T> w;
-            float wf[8];
-            w.load(gate + v * 8);
-            w.unpack(wf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= wf[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            r[i][e] += f[e] * inv;
-            ss += r[i][e] * r[i][e];
-        }
-        rv[i].pack(r[i]);
-        rv[i].store(static_cast<T *>(p.residual_out) + row * p.residual_out_stride + v * 8);
-    }
-    const float inv_r = rsqrtf(row_sum(ss, p.warps_per_row, sums[1]) * p.inv_hidden + p.eps);
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int v = t + i * row_threads;
-        if (!live || v >= p.vecs) continue;
-        Vec8<T> w;
-        float wf[8];
-        w.load(static_cast<const T *>(p.weight) + v * 8);
-        w.unpack(wf);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[i][e] *= inv_r * (wf[e] + p.offset);
-        xv[i].pack(r[i]);
-        xv[i].store(static_cast<T *>(p.out) + row * p.out_stride + v * 8);
-    }
+}
+
+template <typename T, int kVecs>
+int launch_vecs(const NormParams &p, int rows_per_cta, int device, cudaStream_t stream) {
+    const int threads = rows_per_cta * p.warps_per_row * 32;
+    int per_sm = 1;
+    NPD_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, residual_norms_kernel<T, kVecs>, threads, 0));
+    const long long sets = (p.num_rows + rows_per_cta - 1) / rows_per_cta;
+    const long long most = (long long)npd::sm_count(device) * (per_sm > 0 ? per_sm : 1);
+    residual_norms_kernel<T, kVecs><<<static_cast<unsigned>(sets < most ? sets : most), threads, 0, stream>>>(p);
+    NPD_CUDA_TRY(cudaGetLastError());
+    return NPD_OK;
 }
 
 template <typename T>
 int launch(NormParams &p, cudaStream_t stream) {
     int vecs_per_thread = 1;
-    while (vecs_per_thread < 8 && (p.vecs + vecs_per_thread - 1) / vecs_per_thread > kMaxThreads) vecs_per_thread *= 2;
+    while (vecs_per_thread < 8 && (p.vecs + vecs_per_thread - 1) / vecs_per_thread > (vecs_per_thread < 2 ? 256 : kMaxThreads)) vecs_per_thread *= 2;
     p.warps_per_row = ((p.vecs + vecs_per_thread - 1) / vecs_per_thread + 31) / 32;
     const int rows_per_cta = p.warps_per_row >= 4 ? 1 : 4 / p.warps_per_row;
-    const long long grid = (p.num_rows + rows_per_cta - 1) / rows_per_cta;
-    const unsigned g = static_cast<unsigned>(grid), threads = static_cast<unsigned>(rows_per_cta * p.warps_per_row * 32);
-    if (vecs_per_thread == 1) residual_norms_kernel<T, 1><<<g, threads, 0, stream>>>(p);
-    else if (vecs_per_thread == 2) residual_norms_kernel<T, 2><<<g, threads, 0, stream>>>(p);
-    else if (vecs_per_thread == 4) residual_norms_kernel<T, 4><<<g, threads, 0, stream>>>(p);
-    else residual_norms_kernel<T, 8><<<g, threads, 0, stream>>>(p);
-    NPD_CUDA_TRY(cudaGetLastError());
-    return NPD_OK;
+    int dev = 0;
+    NPD_CUDA_TRY(cudaGetDevice(&dev));
+    if (vecs_per_thread == 1) return launch_vecs<T, 1>(p, rows_per_cta, dev, stream);
+    if (vecs_per_thread == 2) return launch_vecs<T, 2>(p, rows_per_cta, dev, stream);
+    if (vecs_per_thread == 4) return launch_vecs<T, 4>(p, rows_per_cta, dev, stream);
+    return launch_vecs<T, 8>(p, rows_per_cta, dev, stream);
 }
 
 }  // namespace

@@ -1,6 +1,6 @@
 // Prompt attention with shaped scores: capped by a tanh, biased by the distance to the key, seen through a sliding window
 // (the formula is in scored_attention.cu; here a query at position i sees the keys i - window < j <= i).  The kernel is the
-// tcgen05 one of prefill_kernel.cuh in its mode kShaped.  A window moves the first key tile of each pair of query tiles, so
+// tcgen05 one of prefill_kernel.cuh in its modes kShaped and kCapped.  A window moves the first key tile of each pair of query tiles, so
 // that the work grows with the window and not with the context.
 #include "prefill_kernel.cuh"
 
@@ -21,7 +21,7 @@ extern "C" int npd_paged_scored_prefill_attention(
     c.slopes = distance_slopes;
     c.window = window;
     try {
-        return run_prefill<kShaped>(c);
+        return score_cap > 0.f ? run_prefill<kCapped>(c) : run_prefill<kShaped>(c);
     } catch (const std::exception &e) {          // the list of work items is host memory
         return npd::fail(NPD_ERR_CUDA, "scored prefill attention: %s", e.what());
     }

@@ -193,6 +193,8 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
                                                  int64_t bt_row_stride, int dtype, void *workspace, size_t workspace_bytes,
                                                  int32_t *status, int flags, void *stream) {
     NPD_REQUIRE((flags & ~0xffff00) == 0, NPD_ERR_INVALID_ARG, "shared-prefix attention: only NPD_FLAG_MAX_CTAS is a flag here");
+    const int rs = npd::check_score_shape("shared-prefix attention", scale, 0.f, nullptr, 0);
+    if (rs != NPD_OK) return rs;
     DecodeCall c{out, q, k_cache, v_cache, block_tables, seq_lens, scale, num_seqs, num_q_heads, num_kv_heads, head_dim,
                  block_size, max_blocks_per_seq, num_blocks, cache_block_stride, bt_row_stride, dtype, workspace,
                  workspace_bytes, flags, stream};

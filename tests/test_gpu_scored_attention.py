@@ -245,3 +245,15 @@ def test_refusals_of_tensors(kernels):
             call(**bad)
     with pytest.raises(RuntimeError, match="takes tensors"):
         kernels.paged_scored_attention(None, q, kc, vc, bt, sl, scale, 16, bt.size(1))
+
+
+@pytest.mark.parametrize("scale", [-0.1, float("nan"), float("inf")])
+def test_scales_that_are_refused(kernels, scale):
+    q, kc, vc, bt, sl, _ = make([20, 3], 12, 2, 128, 16, torch.float16)
+    with pytest.raises(RuntimeError, match="scale"):
+        kernels.paged_scored_attention(torch.empty_like(q), q, kc, vc, bt, sl, scale, 16, bt.size(1), score_cap=5.0)
+
+
+def test_a_scale_of_zero_weighs_every_key_alike(kernels):
+    q, kc, vc, bt, sl, _ = make([20, 300], 12, 2, 128, 16, torch.float16)
+    check(kernels, q, kc, vc, bt, sl, 0.0, 5.0, None, 100)

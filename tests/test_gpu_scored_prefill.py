@@ -199,3 +199,23 @@ def test_refusals(kernels):
                dict(out=q.float()), dict(max_ctas=-1), dict(t=None), dict(toks=5), dict(k=kc[:, :, :8])):
         with pytest.raises(RuntimeError):
             run(**kw)
+
+
+@pytest.mark.parametrize("scale", [-0.1, float("nan"), float("inf")])
+def test_scales_that_are_refused(kernels, scale):
+    q, kc, vc, bt = make([(0, 20)], 12, 2, 128, 16, torch.float16)
+    with pytest.raises(RuntimeError, match="scale"):
+        call(kernels, torch.empty_like(q), q, kc, vc, bt, [(0, 20)], scale, score_cap=5.0)
+
+
+@pytest.mark.parametrize("cap", [1e-9, 1e-3, 1e9])
+def test_caps_far_from_the_usual(kernels, cap):
+    chunks = [(0, 200), (70, 40)]
+    q, kc, vc, bt = make(chunks, 12, 2, 128, 16, torch.float16)
+    if cap > 1:             # scores of 1e9 caps would need their 32 bits for themselves: the cap leaves these as they are
+        out, plain = torch.empty_like(q), torch.empty_like(q)
+        call(kernels, plain, q, kc, vc, bt, chunks, 128 ** -0.5)
+        call(kernels, out, q, kc, vc, bt, chunks, 128 ** -0.5, score_cap=200.0)
+        assert (out.float() - plain.float()).abs().max() <= 2 ** -8
+    else:
+        check(kernels, q, kc, vc, bt, chunks, cap)

@@ -193,3 +193,10 @@ def test_refusals(kernels):
         with pytest.raises(RuntimeError):
             run(**kw)
     kernels.paged_shared_prefix_attention(q[:0], q[:0], kc, vc, bt[:0], sl[:0], go, sh, 0.1, 16, bt.size(1))
+
+
+@pytest.mark.parametrize("scale", [-0.1, float("nan"), float("inf")])
+def test_scales_that_are_refused(kernels, scale):
+    q, kc, vc, bt, sl, go, sh = make([(256, [3, 40, 70])], 12, 2, 128, 16, torch.float16)
+    with pytest.raises(RuntimeError, match="scale"):
+        kernels.paged_shared_prefix_attention(torch.empty_like(q), q, kc, vc, bt, sl, go, sh, scale, 16, bt.size(1))
