@@ -433,58 +433,136 @@ __device__ __forceinline__ float shaped_score(float raw, float slope_log2, int k
     return x + slope_log2 * static_cast<float>(key - pos);
 }
 
-// Joins the prefix pass's pieces for the q heads of (sequence s, virtual kv head h) into `st` (already reduced).
+// Floats of a warp's scratch for write_joined: `group` rows of D values (padded: the writes below are free of bank
+// conflicts) and their maxima and sums.
+__host__ __device__ constexpr int joined_floats(int D, int group) { return group * (D + 4) + 2 * group; }
+
+// kTail: joins the prefix pass's pieces for the q heads of (sequence s, virtual kv head h) with the sequence's own part
+// `st` (already reduced) and writes the rows.  The fragments of `st` go through shared memory into rows, so that a lane
+// reads its 16 bytes of a piece's row with one load and keeps four such pieces of four rows under way: read in the fragments'
+// own layout (4 bytes a load, a quarter of the lanes with heads of their own) the joining took longer than the tail itself.
 template <typename T, int D, int NT>
-__device__ __forceinline__ void fold_prefix(AttnState<T, D, NT> &st, const DecodeParams &p, int s, int h, int lane) {
-    constexpr int KS = D / 16;
+__device__ __forceinline__ void write_joined(const AttnState<T, D, NT> &st, const DecodeParams &p, int s, int h, int lane,
+                                             float *scratch) {
+    constexpr int KS = D / 16, kPitch = D + 4;
+    constexpr int kRowLanes = D / 4;                             // 16-byte pieces of a row
+    constexpr int kRows = 512 / D;                               // rows of one turn: four 16-byte pieces a lane
     const int g = lane >> 2, t4 = lane & 3;
-    const PrefixSeqPlan *sp = p.seq_plan + s;
-    const int key_tiles = __ldcg(&sp->key_tiles);
-    if (key_tiles == 0) return;
-    const int W = __ldcg(&p.plan_head->units_per_worker);
-    const int kv = h / p.kv_rep;
-    const int unit = __ldcg(&sp->unit0) + kv * key_tiles;
-    const int wf = unit / W, wl = (unit + key_tiles - 1) / W;
-    const int first_seq = __ldcg(&sp->item_first_seq), seqs = __ldcg(&sp->item_seqs);
-    const long long row0 = (long long)first_seq * p.num_q_heads + (long long)kv * seqs * p.group_full +
-                           (long long)(p.seq_base + s - first_seq) * p.group_full + (h - kv * p.kv_rep) * p.group;
+    float *ml = scratch + p.group * kPitch;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        // heads past the group read the row of head 0: in bounds, and never written out
-        const int h0 = nt * 8 + 2 * t4, h1 = h0 + 1;
-        const long long r0 = row0 + (h0 < p.group ? h0 : 0), r1 = row0 + (h1 < p.group ? h1 : 0);
-        float m0 = st.m[nt][0], m1 = st.m[nt][1];
-        for (int w = wf; w <= wl; ++w) {
-            m0 = fmaxf(m0, __ldcg(p.prefix_lse + r0 + (long long)w * kPrefixRows));
-            m1 = fmaxf(m1, __ldcg(p.prefix_lse + r1 + (long long)w * kPrefixRows));
-        }
-        const float a0 = fast_exp2(st.m[nt][0] - m0), a1 = fast_exp2(st.m[nt][1] - m1);
-        st.l[nt][0] *= a0;
-        st.l[nt][1] *= a1;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            st.o[nt][j][0] *= a0;
-            st.o[nt][j][1] *= a1;
-            st.o[nt][j][2] *= a0;
-            st.o[nt][j][3] *= a1;
-        }
-        for (int w = wf; w <= wl; ++w) {
-            const long long x0 = r0 + (long long)w * kPrefixRows, x1 = r1 + (long long)w * kPrefixRows;
-            const float w0 = fast_exp2(__ldcg(p.prefix_lse + x0) - m0), w1 = fast_exp2(__ldcg(p.prefix_lse + x1) - m1);
-            st.l[nt][0] += w0;
-            st.l[nt][1] += w1;
-            const float *o0 = p.prefix_o + x0 * D + g, *o1 = p.prefix_o + x1 * D + g;
+        for (int e = 0; e < 2; ++e) {
+            const int head = nt * 8 + 2 * t4 + e;
+            if (head >= p.group) continue;
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-                st.o[nt][j][0] += w0 * __ldcg(o0 + 16 * j);
-                st.o[nt][j][1] += w1 * __ldcg(o1 + 16 * j);
-                st.o[nt][j][2] += w0 * __ldcg(o0 + 16 * j + 8);
-                st.o[nt][j][3] += w1 * __ldcg(o1 + 16 * j + 8);
+                scratch[head * kPitch + 16 * j + g] = st.o[nt][j][e];
+                scratch[head * kPitch + 16 * j + 8 + g] = st.o[nt][j][2 + e];
+            }
+            if (g == 0) {
+                ml[2 * head] = st.m[nt][e];
+                ml[2 * head + 1] = st.l[nt][e];
             }
         }
-        st.m[nt][0] = m0;
-        st.m[nt][1] = m1;
+    __syncwarp();
+
+    const PrefixSeqPlan *sp = p.seq_plan + s;
+    const int key_tiles = __ldcg(&sp->key_tiles);
+    int pieces = 0, wf = 0;
+    long long row0 = 0;                                          // record row of the first head in CTA 0's numbering
+    if (key_tiles > 0) {
+        const int W = __ldcg(&p.plan_head->units_per_worker);
+        const int kv = h / p.kv_rep;
+        const int unit = __ldcg(&sp->unit0) + kv * key_tiles;
+        wf = unit / W;
+        pieces = (unit + key_tiles - 1) / W - wf + 1;
+        const int first_seq = __ldcg(&sp->item_first_seq), seqs = __ldcg(&sp->item_seqs);
+        row0 = (long long)first_seq * p.num_q_heads + (long long)kv * seqs * p.group_full +
+               (long long)(p.seq_base + s - first_seq) * p.group_full + (h - kv * p.kv_rep) * p.group + (long long)wf * kPrefixRows;
     }
+    T *out = static_cast<T *>(p.out) + ((long long)s * p.num_q_heads + (long long)h * p.group) * D;
+    for (int r0 = 0; r0 < p.group; r0 += kRows) {
+        const int rows = min(kRows, p.group - r0);
+        // maxima over the row's parts: lane i looks at piece i (and i + 32, ...)
+        float M[kRows], lse[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            lse[r] = r < rows && lane < pieces ? __ldcg(p.prefix_lse + row0 + r0 + r + (long long)lane * kPrefixRows) : -INFINITY;
+            M[r] = lse[r];
+        }
+        for (int i = lane + 32; i < pieces; i += 32)
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                if (r < rows) M[r] = fmaxf(M[r], __ldcg(p.prefix_lse + row0 + r0 + r + (long long)i * kPrefixRows));
+        float scale[kRows], total[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) M[r] = fmaxf(M[r], __shfl_xor_sync(0xffffffffu, M[r], d));
+            const float m = r < rows ? ml[2 * (r0 + r)] : 0.f;
+            M[r] = fmaxf(M[r], m);
+            scale[r] = fast_exp2(m - M[r]);
+            total[r] = r < rows ? ml[2 * (r0 + r) + 1] * scale[r] : 1.f;
+        }
+        // a lane's piece q of this turn: row (q * 32 + lane) / kRowLanes, 16-byte column (q * 32 + lane) % kRowLanes
+        float4 acc[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = (q * 32 + lane) / kRowLanes, c = (q * 32 + lane) % kRowLanes;
+            acc[q] = r < rows ? *reinterpret_cast<const float4 *>(scratch + (r0 + r) * kPitch + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float f = scale[0];
+#pragma unroll
+            for (int x = 1; x < kRows; ++x) f = r == x ? scale[x] : f;
+            acc[q].x *= f, acc[q].y *= f, acc[q].z *= f, acc[q].w *= f;
+        }
+        for (int i0 = 0; i0 < pieces; i0 += 32) {
+            if (i0 > 0) {
+#pragma unroll
+                for (int r = 0; r < kRows; ++r)
+                    lse[r] = r < rows && i0 + lane < pieces ? __ldcg(p.prefix_lse + row0 + r0 + r + (long long)(i0 + lane) * kPrefixRows) : -INFINITY;
+            }
+            float wt[kRows];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                wt[r] = fast_exp2(lse[r] - M[r]);
+                float sum = wt[r];
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                total[r] += sum;
+            }
+            const int n = min(32, pieces - i0);
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const float *piece = p.prefix_o + (row0 + r0 + (long long)(i0 + i) * kPrefixRows) * D;
+                float w[kRows];
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) w[r] = __shfl_sync(0xffffffffu, wt[r], i);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = (q * 32 + lane) / kRowLanes;
+                    if (r >= rows) continue;
+                    float f = w[0];
+#pragma unroll
+                    for (int x = 1; x < kRows; ++x) f = r == x ? w[x] : f;
+                    const float4 o = __ldcg(reinterpret_cast<const float4 *>(piece) + q * 32 + lane);
+                    acc[q].x += f * o.x, acc[q].y += f * o.y, acc[q].z += f * o.z, acc[q].w += f * o.w;
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = (q * 32 + lane) / kRowLanes, c = (q * 32 + lane) % kRowLanes;
+            if (r >= rows) continue;
+            float f = total[0];
+#pragma unroll
+            for (int x = 1; x < kRows; ++x) f = r == x ? total[x] : f;
+            const float inv = 1.f / f;
+            const uint2 v = make_uint2(Elem<T>::pack2(acc[q].x * inv, acc[q].y * inv), Elem<T>::pack2(acc[q].z * inv, acc[q].w * inv));
+            *reinterpret_cast<uint2 *>(out + (long long)(r0 + r) * D + 4 * c) = v;
+        }
+    }
+    __syncwarp();                                                // the scratch is free for the next (sequence, kv head)
 }
 
 // ---------------------------------------------------------------------------
@@ -529,6 +607,9 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
     uint8_t *stage_base = sbase + (size_t)warp * nst * STAGE_BYTES;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sbase + (size_t)nwarps * nst * STAGE_BYTES) + warp * nst;
     int *pre = reinterpret_cast<int *>(sbase + (size_t)nwarps * nst * (STAGE_BYTES + 8));
+    float *scratch = nullptr;        // kTail: this warp's rows on their way out
+    if (MODE == kTail)
+        scratch = reinterpret_cast<float *>(pre + (p.num_seqs + 4) / 4 * 4) + warp * ((joined_floats(D, p.group) + 3) / 4 * 4);
 
     if (lane == 0) {
         for (int i = 0; i < nst; ++i) mbar_init(smem_u32(bars + i), 1);
@@ -538,6 +619,7 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
     }
+    if (MODE == kTail) asm volatile("griddepcontrol.wait;" ::: "memory");     // the plan and the pieces are complete
     long long W = 0;
     int worker = 0, my_tiles = 0;
     Cursor pc, cc;                   // producer / consumer cursors over the same range
@@ -843,8 +925,8 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
             // this warp's run is done and nothing is in flight into its ring: the record goes there
             write_partial<T, D, NT>(st, reinterpret_cast<float *>(stage_base), lane);
         } else if (!head_cut && !tail_cut) {
-            if (MODE == kTail) fold_prefix<T, D, NT>(st, p, seg_s, seg_h, lane);
-            write_output<T, D, NT>(st, p, seg_s, seg_h, lane);
+            if (MODE == kTail) write_joined<T, D, NT>(st, p, seg_s, seg_h, lane, scratch);
+            else write_output<T, D, NT>(st, p, seg_s, seg_h, lane);
         } else {
             float *rec = p.partials + ((size_t)worker * 2 + (head_cut ? 0 : 1)) * rec_floats<D, NT>();
             write_partial<T, D, NT>(st, rec, lane);
@@ -862,8 +944,8 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
                 if (ticket == wl - wf) {
                     __threadfence();                   // the other workers' records are visible to me
                     merge_partials<T, D, NT>(st, p, wf, wl, lane);
-                    if (MODE == kTail) fold_prefix<T, D, NT>(st, p, seg_s, seg_h, lane);
-                    write_output<T, D, NT>(st, p, seg_s, seg_h, lane);
+                    if (MODE == kTail) write_joined<T, D, NT>(st, p, seg_s, seg_h, lane, scratch);
+                    else write_output<T, D, NT>(st, p, seg_s, seg_h, lane);
                     if (lane == 0) *slot = 0;          // ready for the next launch
                 }
             }
@@ -970,15 +1052,43 @@ int choose_kv_rep(int group, int max_heads) {
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+constexpr size_t kMaxSmem = 227 * 1024;
+size_t tail_smem(int head_dim, int group, const LaunchShape &ls, int64_t num_seqs) {
+    const size_t stage_bytes = 2 * kTile * (size_t)head_dim * 2;
+    return 1024 + (size_t)ls.nwarps * ls.nstages * (stage_bytes + 8) + ((size_t)num_seqs + 1) * 4 + 32 +
+           (size_t)ls.nwarps * ((joined_floats(head_dim, group) + 3) / 4 * 4) * sizeof(float);
+}
+
 template <int MODE, typename T, int D, int NT, bool IL>
 int launch_decode(const DecodeParams &p, const CUtensorMap &tk, const CUtensorMap &tv, const LaunchShape &ls,
                   cudaStream_t stream) {
     constexpr int STAGE_BYTES = 2 * kTile * D * 2;
-    const size_t smem = 1024 + (size_t)ls.nwarps * ls.nstages * (STAGE_BYTES + 8) + ((size_t)p.num_seqs + 1) * 4 + 16;
+    const size_t smem = MODE == kTail ? tail_smem(D, p.group, ls, p.num_seqs)
+                                      : 1024 + (size_t)ls.nwarps * ls.nstages * (STAGE_BYTES + 8) + ((size_t)p.num_seqs + 1) * 4 + 16;
+    if constexpr (MODE == kTail) {
+        // launched while the prefix pass still runs; waits for it before it reads anything that it or the plan wrote
+        auto launch = [&](auto kern) -> int {
+            NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(ls.grid);
+            cfg.blockDim = dim3(ls.nwarps * 32);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream = stream;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = p.seq_base == 0 ? 1 : 0;              // a second sub-batch follows the first in full
+            NPD_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, tk, tv));
+            return NPD_OK;
+        };
+        if (ls.nwarps <= 8) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>);
+        return launch(paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>);
+    } else {
     // Largest shared-memory carve-out on both instances: the SM then has room for a small CTA of another stream
     // (the page migration kernel asks for the same), instead of being configured for this CTA alone.
     if (ls.small) {
-        if constexpr (!IL && MODE != kTail) {
+        if constexpr (!IL) {
             auto kern = paged_decode_stream_kernel<T, D, NT, false, 8, true, MODE>;
             NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
@@ -997,6 +1107,7 @@ int launch_decode(const DecodeParams &p, const CUtensorMap &tk, const CUtensorMa
     }
     NPD_CUDA_TRY(cudaGetLastError());
     return NPD_OK;
+    }
 }
 
 template <int MODE, typename T, bool IL>
@@ -1099,6 +1210,12 @@ int run_decode(const DecodeCall &c) {
                         (c.flags & NPD_DECODE_KV_INTERLEAVED) != 0, c.flags, dev);
     NPD_REQUIRE((reinterpret_cast<uintptr_t>(c.workspace) & 255u) == 0, NPD_ERR_WORKSPACE,
                 "decode attention: workspace must be 256-byte aligned");
+    if (MODE == kTail) {
+        // the joined rows' scratch shares the CTA's memory with the rings: fewer stages, then fewer warps, where both do not fit
+        auto bytes = [&] { return tail_smem(static_cast<int>(c.head_dim), wp.group, ls, c.num_seqs < kMaxSeqsPerLaunch ? c.num_seqs : kMaxSeqsPerLaunch); };
+        while (bytes() > kMaxSmem && ls.nstages > 1) --ls.nstages;
+        while (bytes() > kMaxSmem && ls.nwarps > 4) ls.nwarps -= 4;
+    }
 
     CUtensorMap tk, tv;
     const int box_rows = c.block_size < 16 ? static_cast<int>(c.block_size) : 16;

@@ -550,6 +550,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         ctrl->abort_flag = 0;
         mbar_fence_init();
     }
+    if (MODE == kPrefix) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 9) {
         tmem_alloc(smem_u32(&ctrl->tmem_base), kTmemCols);
         tmem_relinquish();
@@ -603,6 +604,8 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         bool ok = true;
         PrefixRun run{};
         if (MODE == kPrefix && k_role) {
+            // this kernel is launched while the plan is made; everything that depends on the plan passes through this warp
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             run.at = p.seeds[blockIdx.x];
             run.left = min(p.plan->units_per_worker, p.plan->total_units - static_cast<int>(blockIdx.x) * p.plan->units_per_worker);
         }

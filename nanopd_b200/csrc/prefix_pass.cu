@@ -23,7 +23,16 @@ int npd::launch_prefix_pass(const PrefixPass &a) {
     p.plan = static_cast<const PrefixPlanHead *>(a.plan_head);
     p.prefix_o = a.prefix_o;
     p.prefix_lse = a.prefix_lse;
-    l.kernel<<<static_cast<unsigned>(a.ctas), kThreads, l.smem, static_cast<cudaStream_t>(a.stream)>>>(p, l.q, l.k, l.v);
-    NPD_CUDA_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.ctas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = l.smem;
+    cfg.stream = static_cast<cudaStream_t>(a.stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // set up while the plan kernel runs
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NPD_CUDA_TRY(cudaLaunchKernelEx(&cfg, l.kernel, p, l.q, l.k, l.v));
     return NPD_OK;
 }

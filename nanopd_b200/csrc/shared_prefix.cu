@@ -69,43 +69,58 @@ __device__ void exclusive_prefix(int *v, int n) {
 
 __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const PlanParams p) {
     extern __shared__ int plan_smem[];
-    int *unit = plan_smem;                       // [num_groups + 1] units in front of each group
+    int *offs = plan_smem;                       // [num_groups + 1] group_offsets
+    int *unit = offs + p.num_groups + 1;         // [num_groups + 1] units in front of each group
+    int *least = unit + p.num_groups + 1;        // [num_groups] shortest sequence that is not empty
     __shared__ int bad, units_per_worker;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int my_len = tid < p.num_seqs ? p.seq_lens[tid] : 0;      // under way together with the offsets
     if (tid == 0) bad = 0;
+    for (int g = tid; g <= p.num_groups; g += kPlanThreads) {
+        offs[g] = p.group_offsets[g];
+        if (g < p.num_groups) least[g] = INT32_MAX;
+    }
     __syncthreads();
     // Groups must be consecutive ranges of the batch.  Anything else shares nothing (every row is still right: the tail
     // then covers whole sequences) and is flagged.
-    for (int g = tid; g < p.num_groups; g += kPlanThreads) {
-        const int a = p.group_offsets[g], b = p.group_offsets[g + 1];
-        if (a < 0 || b < a || b > p.num_seqs) bad = 1;
+    for (int g = tid; g < p.num_groups; g += kPlanThreads)
+        if (offs[g] < 0 || offs[g + 1] < offs[g] || offs[g + 1] > p.num_seqs) bad = 1;
+    __syncthreads();
+    const bool none = bad != 0;
+    if (none && tid == 0) atomicOr(p.status, NPD_STATUS_BAD_POSITION);
+    // the last group that begins at or before sequence s, or -1
+    auto group_of = [&](int s) {
+        if (none || s < offs[0] || s >= offs[p.num_groups]) return -1;
+        int lo = 0, hi = p.num_groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (offs[mid] <= s) lo = mid; else hi = mid - 1;
+        }
+        return lo;
+    };
+    for (int s = tid; s < p.num_seqs; s += kPlanThreads) {
+        const int n = s == tid ? my_len : p.seq_lens[s];
+        const int g = group_of(s);
+        if (g >= 0 && n > 0) atomicMin(least + g, n);
     }
     __syncthreads();
-    if (bad && tid == 0) atomicOr(p.status, NPD_STATUS_BAD_POSITION);
-    for (int g = warp; g < p.num_groups; g += kPlanThreads / 32) {
+    for (int g = tid; g < p.num_groups; g += kPlanThreads) {
         PrefixGroup out{0, 0, 0, 0};
-        if (!bad) {
-            out.begin = p.group_offsets[g];
-            out.seqs = p.group_offsets[g + 1] - out.begin;
-            int least = INT32_MAX;               // shortest sequence that is not empty
-            for (int i = lane; i < out.seqs; i += 32) {
-                const int n = p.seq_lens[out.begin + i];
-                if (n > 0) least = min(least, n);
-            }
-            least = __reduce_min_sync(0xffffffffu, least);
+        if (!none) {
+            out.begin = offs[g];
+            out.seqs = offs[g + 1] - offs[g];
             const int shared = p.shared_lens[g];
-            if (shared < 0 && lane == 0) atomicOr(p.status, NPD_STATUS_BAD_POSITION);
+            if (shared < 0) atomicOr(p.status, NPD_STATUS_BAD_POSITION);
             // at least one token stays with each sequence, so that the tail kernel visits (and writes) every row
-            if (out.seqs > 1 && least != INT32_MAX) {
-                const long long most = min((long long)least, p.cap) - 1;
+            if (out.seqs > 1 && least[g] != INT32_MAX) {
+                const long long most = min((long long)least[g], p.cap) - 1;
                 out.tokens = static_cast<int>(min((long long)max(shared, 0), most)) / kTile * kTile;
             }
             out.key_tiles = (out.tokens + p.tile_keys - 1) / p.tile_keys;
         }
-        if (lane == 0) {
-            p.groups[g] = out;
-            unit[g] = out.key_tiles * ((out.seqs + p.item_seqs - 1) / p.item_seqs) * p.num_kv_heads;
-        }
+        p.groups[g] = out;
+        unit[g] = out.key_tiles * ((out.seqs + p.item_seqs - 1) / p.item_seqs) * p.num_kv_heads;
     }
     __syncthreads();
     exclusive_prefix(unit, p.num_groups);
@@ -117,12 +132,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     __syncthreads();
     for (int s = tid; s < p.num_seqs; s += kPlanThreads) {
         PrefixSeqPlan sp{0, 0, 0, 0, 0, {0, 0, 0}};
-        if (!bad && s >= p.group_offsets[0] && s < p.group_offsets[p.num_groups]) {
-            int lo = 0, hi = p.num_groups - 1;   // the last group that begins at or before s
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (p.group_offsets[mid] <= s) lo = mid; else hi = mid - 1;
-            }
+        const int lo = group_of(s);
+        if (lo >= 0) {
             const PrefixGroup g = p.groups[lo];
             const int item = (s - g.begin) / p.item_seqs;
             sp.first_tile = g.tokens / kTile;
@@ -235,7 +246,9 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
     pp.tile_keys = tile_keys;
     pp.workers = cap > 0 && cap < sms ? cap : sms;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    shared_prefix_plan_kernel<<<1, kPlanThreads, (size_t)(num_groups + 1) * sizeof(int), st>>>(pp);
+    constexpr size_t plan_most = (size_t)(3 * kMaxGroups + 2) * sizeof(int);
+    NPD_CUDA_TRY(cudaFuncSetAttribute(shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_most));
+    shared_prefix_plan_kernel<<<1, kPlanThreads, (size_t)(3 * num_groups + 2) * sizeof(int), st>>>(pp);
     NPD_CUDA_TRY(cudaGetLastError());
     npd::PrefixPass pass{q, k_cache, v_cache, block_tables, scale, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
                          max_blocks_per_seq, num_blocks, cache_block_stride, bt_row_stride, dtype, status, pp.groups, pp.seeds,

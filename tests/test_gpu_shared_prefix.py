@@ -200,3 +200,22 @@ def test_scales_that_are_refused(kernels, scale):
     q, kc, vc, bt, sl, go, sh = make([(256, [3, 40, 70])], 12, 2, 128, 16, torch.float16)
     with pytest.raises(RuntimeError, match="scale"):
         kernels.paged_shared_prefix_attention(torch.empty_like(q), q, kc, vc, bt, sl, go, sh, scale, 16, bt.size(1))
+
+
+def test_the_largest_batches(kernels):
+    """4096 groups of one, two and three, and a batch that takes two sub-batches of the tail."""
+    groups = [(16 * (i % 3), [1 + (i + j) % 20 for j in range(1 + i % 3)]) for i in range(4096)]
+    state = make(groups, 4, 1, 64, 16, torch.float16)
+    q, kc, vc, bt, sl, go, sh = state
+    assert q.size(0) > 8000
+    out = torch.full_like(q, float("nan"))
+    call(kernels, out, *state)
+    plain = torch.empty_like(q)
+    kernels.paged_attention_forward(plain, q, kc, vc, bt, sl, 0.125, 16, bt.size(1))
+    assert (out.float() - plain.float()).abs().max() <= 2 ** -9
+    state = make([(1600, [1 + i % 30 for i in range(4100)])], 4, 1, 64, 16, torch.float16)
+    q, kc, vc, bt, sl, go, sh = state
+    out, plain = torch.full_like(q, float("nan")), torch.empty_like(q)
+    call(kernels, out, *state)
+    kernels.paged_attention_forward(plain, q, kc, vc, bt, sl, 0.125, 16, bt.size(1))
+    assert (out.float() - plain.float()).abs().max() <= 2 ** -9
