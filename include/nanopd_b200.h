@@ -325,6 +325,18 @@ int npd_residual_norms(void *residual_out, void *out, const void *x, const void 
                        int64_t gate_row_stride, int64_t residual_out_row_stride,
                        int64_t out_row_stride, int dtype, void *stream);
 
+/* ---- the same calls with packed arguments -------------------------------------------------
+ * For hosts that pay for every argument of a foreign call (a ctypes call of (7) spends more on
+ * its 25 arguments than on the launch): `slots` holds the device to launch on, then the
+ * arguments of the operator's entry point above in their order, one 8-byte slot each, pointers
+ * and integers as 64-bit integers and floats as doubles.  The device is made current for the call. */
+#define NPD_OP_SCORED_ATTENTION          7
+#define NPD_OP_SCORED_PREFILL_ATTENTION  8
+#define NPD_OP_SHARED_PREFIX_ATTENTION   9
+#define NPD_OP_RESIDUAL_NORMS           10
+typedef union { int64_t i; uint64_t u; double f; } npd_slot;
+int npd_call_packed(int op, const npd_slot *slots);
+
 /* Enables peer access from the current device to `peer_device` (idempotent).
  * Stands in for the driver-side mapping torch's copy_ sets up in the reference
  * (nanoPD/workers/kv_transfer.py:6-14 only probes can_device_access_peer).              */

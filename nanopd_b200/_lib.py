@@ -12,6 +12,7 @@ NPD_ERR_INVALID_ARG, NPD_ERR_UNSUPPORTED, NPD_ERR_CUDA, NPD_ERR_WORKSPACE = 1, 2
 NPD_DTYPE_F16, NPD_DTYPE_BF16, NPD_DTYPE_F32 = 0, 1, 2
 NPD_STATUS_BAD_BLOCK_ID, NPD_STATUS_BAD_POSITION, NPD_STATUS_WAIT_TIMEOUT = 1, 2, 4
 NPD_DECODE_KV_INTERLEAVED = 2
+NPD_OP_SCORED_ATTENTION, NPD_OP_SCORED_PREFILL_ATTENTION, NPD_OP_SHARED_PREFIX_ATTENTION, NPD_OP_RESIDUAL_NORMS = 7, 8, 9, 10
 
 # name -> (restype, argtypes); the order mirrors include/nanopd_b200.h
 SIGNATURES = {
@@ -55,6 +56,7 @@ SIGNATURES = {
     "npd_paged_shared_prefix_attention": (c_int, [c_void_p] * 8 + [c_float] + [c_int64] * 10 +
                                           [c_int, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
     "npd_residual_norms": (c_int, [c_void_p] * 7 + [c_float] * 3 + [c_int64] * 7 + [c_int, c_void_p]),
+    "npd_call_packed": (c_int, [c_int, c_char_p]),
     "npd_enable_peer_access": (c_int, [c_int]),
 }
 

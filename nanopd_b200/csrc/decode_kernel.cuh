@@ -69,6 +69,7 @@ struct DecodeParams {
     long long bt_row_stride;
     int num_workers;
     int num_stages;
+    int seg_cost;         // see unit_at; kScored and kTail
     // kScored: scores are shaped before the softmax (all in the log2 domain)
     float cap_in;         // 2 log2(e) * scale / cap, the exponent's factor in tanh; 0 = scores are not capped
     float cap_log2;       // cap * log2(e)
@@ -177,6 +178,31 @@ struct Cursor {
     int len;       // clamped length of sequence s
     int first;     // its first tile
 };
+
+// The line that is cut into equal ranges holds, for every (sequence, virtual kv head), its tiles and then p.seg_cost
+// further units that stand for what a (sequence, kv head) costs beside its tiles: fetching its query rows, merging, writing.
+// Without them a range over short sequences takes several times as long as one over a long sequence.  kPlain counts tiles
+// alone.  unit_at: first unit of (s, h); tiles_before: tiles in front of unit f.
+template <int MODE>
+__device__ __forceinline__ long long unit_at(int s, int h, const int *pre, const DecodeParams &p) {
+    const int n = pre[s + 1] - pre[s];
+    if (MODE == kPlain) return (long long)p.num_vheads * pre[s] + (long long)h * n;
+    return (long long)p.num_vheads * (pre[s] + (long long)p.seg_cost * s) + (long long)h * (n + p.seg_cost);
+}
+template <int MODE>
+__device__ long long tiles_before(long long f, const int *pre, const DecodeParams &p) {
+    if (MODE == kPlain) return f;
+    int lo = 0, hi = p.num_seqs;                 // the last s in [0, num_seqs] whose units begin at or before f
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((long long)p.num_vheads * (pre[mid] + (long long)p.seg_cost * mid) <= f) lo = mid; else hi = mid - 1;
+    }
+    if (lo == p.num_seqs) return (long long)p.num_vheads * pre[lo];
+    const int n = pre[lo + 1] - pre[lo];
+    const int r = static_cast<int>(f - (long long)p.num_vheads * (pre[lo] + (long long)p.seg_cost * lo));
+    const int h = r / (n + p.seg_cost), t = r - h * (n + p.seg_cost);
+    return (long long)p.num_vheads * pre[lo] + (long long)h * n + min(t, n);
+}
 
 template <int MODE>
 __device__ __forceinline__ void cursor_seek(Cursor &c, long long f, const int *pre, const DecodeParams &p) {
@@ -654,12 +680,18 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
             for (int i = threadIdx.x; i < p.num_q_heads * D / 2; i += blockDim.x) row[i] = 0u;
         }
 
-        const long long total = (long long)p.num_vheads * pre[p.num_seqs];
+        const long long total = MODE == kPlain ? (long long)p.num_vheads * pre[p.num_seqs]
+                                               : (long long)p.num_vheads * (pre[p.num_seqs] + (long long)p.seg_cost * p.num_seqs);
         W = tiles_per_worker(total, p.num_workers, (long long)p.num_vheads * p.num_seqs);
         worker = blockIdx.x * nwarps + warp;
-        const long long f_begin = (long long)worker * W;
+        long long f_begin = (long long)worker * W;
         if (f_begin >= total) return;
-        const long long f_end = min(f_begin + W, total);
+        long long f_end = min(f_begin + W, total);
+        if (MODE != kPlain) {
+            f_begin = tiles_before<MODE>(f_begin, pre, p);
+            f_end = tiles_before<MODE>(f_end, pre, p);
+            if (f_begin >= f_end) return;
+        }
         my_tiles = static_cast<int>(f_end - f_begin);
         cursor_seek<MODE>(pc, f_begin, pre, p);
     }
@@ -933,7 +965,7 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
             if (!p.skip_merge) {
                 // Which workers share this (sequence, kv head)?  The one whose ticket is the last merges.
                 const int n_s = pre[seg_s + 1] - pre[seg_s];
-                const long long fb = (long long)p.num_vheads * pre[seg_s] + (long long)seg_h * n_s;
+                const long long fb = unit_at<MODE>(seg_s, seg_h, pre, p);
                 const int wf = static_cast<int>(fb / W), wl = static_cast<int>((fb + n_s - 1) / W);
                 __threadfence();                       // every lane: my part of the record is visible device-wide
                 __syncwarp();
@@ -1052,7 +1084,7 @@ int choose_kv_rep(int group, int max_heads) {
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
-constexpr size_t kMaxSmem = 227 * 1024;
+constexpr int kDecodeMaxSmem = npd::kMaxDynamicSmem - 1024;      // the kernel has some static shared memory too
 size_t tail_smem(int head_dim, int group, const LaunchShape &ls, int64_t num_seqs) {
     const size_t stage_bytes = 2 * kTile * (size_t)head_dim * 2;
     return 1024 + (size_t)ls.nwarps * ls.nstages * (stage_bytes + 8) + ((size_t)num_seqs + 1) * 4 + 32 +
@@ -1067,8 +1099,13 @@ int launch_decode(const DecodeParams &p, const CUtensorMap &tk, const CUtensorMa
                                       : 1024 + (size_t)ls.nwarps * ls.nstages * (STAGE_BYTES + 8) + ((size_t)p.num_seqs + 1) * 4 + 16;
     if constexpr (MODE == kTail) {
         // launched while the prefix pass still runs; waits for it before it reads anything that it or the plan wrote
-        auto launch = [&](auto kern) -> int {
-            NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        auto launch = [&](auto kern, std::atomic<unsigned long long> &done) -> int {
+            int dev = 0;
+            NPD_CUDA_TRY(cudaGetDevice(&dev));
+            if (npd::first_on_device(done, dev)) {
+                NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecodeMaxSmem));
+                npd::set_up_on_device(done, dev);
+            }
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(ls.grid);
             cfg.blockDim = dim3(ls.nwarps * 32);
@@ -1082,31 +1119,50 @@ int launch_decode(const DecodeParams &p, const CUtensorMap &tk, const CUtensorMa
             NPD_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, tk, tv));
             return NPD_OK;
         };
-        if (ls.nwarps <= 8) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>);
-        return launch(paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>);
+        static std::atomic<unsigned long long> done8{0}, done12{0};
+        if (ls.nwarps <= 8) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>, done8);
+        return launch(paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>, done12);
+    } else if constexpr (MODE == kScored) {
+        // every instance: the largest shared-memory carve-out (see below), set once per device
+        auto launch = [&](auto kern, std::atomic<unsigned long long> &done) -> int {
+            int dev = 0;
+            NPD_CUDA_TRY(cudaGetDevice(&dev));
+            if (npd::first_on_device(done, dev)) {
+                NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecodeMaxSmem));
+                NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+                npd::set_up_on_device(done, dev);
+            }
+            kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
+            NPD_CUDA_TRY(cudaGetLastError());
+            return NPD_OK;
+        };
+        static std::atomic<unsigned long long> done_small{0}, done8{0}, done12{0};
+        if (ls.small) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, true, MODE>, done_small);
+        if (ls.nwarps <= 8) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>, done8);
+        return launch(paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>, done12);
     } else {
-    // Largest shared-memory carve-out on both instances: the SM then has room for a small CTA of another stream
-    // (the page migration kernel asks for the same), instead of being configured for this CTA alone.
-    if (ls.small) {
-        if constexpr (!IL) {
-            auto kern = paged_decode_stream_kernel<T, D, NT, false, 8, true, MODE>;
+        // Largest shared-memory carve-out on both instances: the SM then has room for a small CTA of another stream
+        // (the page migration kernel asks for the same), instead of being configured for this CTA alone.
+        if (ls.small) {
+            if constexpr (!IL) {
+                auto kern = paged_decode_stream_kernel<T, D, NT, false, 8, true>;
+                NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+                kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
+            }
+        } else if (ls.nwarps <= 8) {
+            auto kern = paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>;
+            NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+            kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
+        } else {
+            auto kern = paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>;
             NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
             kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
         }
-    } else if (ls.nwarps <= 8) {
-        auto kern = paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>;
-        NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-        kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
-    } else {
-        auto kern = paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>;
-        NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-        kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
-    }
-    NPD_CUDA_TRY(cudaGetLastError());
-    return NPD_OK;
+        NPD_CUDA_TRY(cudaGetLastError());
+        return NPD_OK;
     }
 }
 
@@ -1198,6 +1254,9 @@ int run_decode(const DecodeCall &c) {
     NPD_CUDA_TRY(cudaGetDevice(&dev));
     LaunchShape ls = launch_shape(static_cast<int>(c.head_dim), static_cast<int>(c.block_size), (c.flags >> 8) & 0xffff,
                                   (long long)c.num_seqs * c.num_kv_heads, dev);
+    // The shaping of a tile's scores and the joining of pieces lengthen a warp's chain per tile: where plain scores take 8
+    // warps, these take 12 (256 ragged sequences, capped: 241 us against 248; behind 8192 shared tokens: 128 against 131)
+    if (MODE != kPlain && c.head_dim == 128 && ls.nstages == 2 && ls.nwarps == 8) ls.nwarps = NPD_DECODE_MAX_WARPS;
     const WorkspacePlan wp = plan_workspace(c.num_seqs, c.num_q_heads, c.num_kv_heads, c.head_dim, ls);
     NPD_REQUIRE(c.workspace != nullptr && c.workspace_bytes >= wp.total, NPD_ERR_WORKSPACE,
                 "decode attention: workspace of %zu bytes given, %zu needed", c.workspace_bytes, wp.total);
@@ -1213,8 +1272,8 @@ int run_decode(const DecodeCall &c) {
     if (MODE == kTail) {
         // the joined rows' scratch shares the CTA's memory with the rings: fewer stages, then fewer warps, where both do not fit
         auto bytes = [&] { return tail_smem(static_cast<int>(c.head_dim), wp.group, ls, c.num_seqs < kMaxSeqsPerLaunch ? c.num_seqs : kMaxSeqsPerLaunch); };
-        while (bytes() > kMaxSmem && ls.nstages > 1) --ls.nstages;
-        while (bytes() > kMaxSmem && ls.nwarps > 4) ls.nwarps -= 4;
+        while (bytes() > (size_t)kDecodeMaxSmem && ls.nstages > 1) --ls.nstages;
+        while (bytes() > (size_t)kDecodeMaxSmem && ls.nwarps > 4) ls.nwarps -= 4;
     }
 
     CUtensorMap tk, tv;
@@ -1267,6 +1326,7 @@ int run_decode(const DecodeCall &c) {
     p.cap_log2 = c.score_cap * 1.4426950408889634f;
     p.slopes = c.slopes;
     p.window = c.window > 0 && c.window < INT32_MAX ? static_cast<int>(c.window) : INT32_MAX;
+    p.seg_cost = MODE == kTail ? 6 : 2;
     p.plan_head = c.plan_head;
     p.prefix_o = c.prefix_o;
     p.prefix_lse = c.prefix_lse;

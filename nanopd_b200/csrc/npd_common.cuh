@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -64,6 +65,16 @@ int encode_tiled_3d(CUtensorMap *map, const void *base, int dtype, const uint64_
 int encode_cache_tensor_map(CUtensorMap *map, const void *base, int dtype, int64_t head_dim,
                             int64_t rows_per_block, int64_t num_blocks,
                             int64_t block_stride_elems, int box_rows);
+
+// Function attributes that a kernel needs once per device: `done` is a static of the kernel's launcher, one bit a device.
+// True when this device still has to be set up.
+inline bool first_on_device(std::atomic<unsigned long long> &done, int device) {
+    return device < 0 || device >= 64 || !(done.load(std::memory_order_acquire) >> device & 1ull);
+}
+inline void set_up_on_device(std::atomic<unsigned long long> &done, int device) {
+    if (device >= 0 && device < 64) done.fetch_or(1ull << device, std::memory_order_release);
+}
+constexpr int kMaxDynamicSmem = 227 * 1024;
 
 // Checks of the arguments that shape scores, the same for decode and prompts.
 int check_score_shape(const char *op, float scale, float score_cap, const float *distance_slopes, int64_t window);

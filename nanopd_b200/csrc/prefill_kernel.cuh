@@ -1238,7 +1238,15 @@ int prepare_launch(const PrefillCall &c, int64_t total_tokens, PrefillLaunch &l)
     else NPD_PICK(256);
 #undef NPD_PICK
 #undef NPD_PICK_B
-    NPD_CUDA_TRY(cudaFuncSetAttribute(l.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.smem));
+    // once per device and instance (head size, type, box height)
+    static std::atomic<unsigned long long> done[18];
+    const int instance = ((c.head_dim == 64 ? 0 : (c.head_dim == 128 ? 1 : 2)) * 2 + (f16 ? 1 : 0)) * 3 + (l.box_rows == 4 ? 0 : (l.box_rows == 8 ? 1 : 2));
+    int dev = 0;
+    NPD_CUDA_TRY(cudaGetDevice(&dev));
+    if (npd::first_on_device(done[instance], dev)) {
+        NPD_CUDA_TRY(cudaFuncSetAttribute(l.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, npd::kMaxDynamicSmem));
+        npd::set_up_on_device(done[instance], dev);
+    }
     return NPD_OK;
 }
 

@@ -288,10 +288,15 @@ template <typename T, int kVecs, bool kStaged>
 int launch_kernel(const NormParams &p, int rows_per_cta, size_t smem, int device, cudaStream_t stream) {
     auto kern = residual_norms_kernel<T, kVecs, kStaged>;
     const int threads = rows_per_cta * p.warps_per_row * 32;
-    NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRing));
-    NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    int per_sm = 1;
-    NPD_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem));
+    static std::atomic<unsigned long long> done{0};
+    if (npd::first_on_device(done, device)) {
+        NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRing));
+        NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+        npd::set_up_on_device(done, device);
+    }
+    // resident CTAs: by the register limit of the kernel's declaration and by the ring (the rest follows from these two)
+    const int by_registers = 65536 / ((kVecs <= kHeld ? 96 : 128) * threads), by_ring = static_cast<int>((size_t)npd::kMaxDynamicSmem / (smem + 1280));
+    const int per_sm = by_registers < by_ring ? by_registers : by_ring;
     const long long sets = (p.num_rows + rows_per_cta - 1) / rows_per_cta;
     const long long most = (long long)npd::sm_count(device) * (per_sm > 0 ? per_sm : 1);
     kern<<<static_cast<unsigned>(sets < most ? sets : most), threads, smem, stream>>>(p);

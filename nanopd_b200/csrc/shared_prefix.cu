@@ -247,7 +247,11 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
     pp.workers = cap > 0 && cap < sms ? cap : sms;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     constexpr size_t plan_most = (size_t)(3 * kMaxGroups + 2) * sizeof(int);
-    NPD_CUDA_TRY(cudaFuncSetAttribute(shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_most));
+    static std::atomic<unsigned long long> plan_done{0};
+    if (npd::first_on_device(plan_done, dev)) {
+        NPD_CUDA_TRY(cudaFuncSetAttribute(shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_most));
+        npd::set_up_on_device(plan_done, dev);
+    }
     shared_prefix_plan_kernel<<<1, kPlanThreads, (size_t)(3 * num_groups + 2) * sizeof(int), st>>>(pp);
     NPD_CUDA_TRY(cudaGetLastError());
     npd::PrefixPass pass{q, k_cache, v_cache, block_tables, scale, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,

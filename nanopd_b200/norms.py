@@ -7,15 +7,17 @@ decode harness calls it for layers of that shape (``decoder_step.DecoderShape.po
 """
 from __future__ import annotations
 
+import struct
 from typing import Dict, Optional
 
 import torch
 
-from . import _lib
-from .paged_kernels import _DTYPE_CODE, _C, _call, _raw_stream, _remember, _require, _sig
+from ._lib import NPD_OP_RESIDUAL_NORMS
+from .paged_kernels import _DTYPE_CODE, _packed_op, _raw_stream, _remember, _require
 
 MAX_HIDDEN = 32768
 _plans: Dict[tuple, tuple] = {}
+_pack = struct.Struct("<q7Q3d8qQ").pack                # device, then the entry point's arguments
 
 
 def _rows(t: torch.Tensor, name: str, T: int, H: int) -> int:
@@ -47,8 +49,13 @@ def residual_norms(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor
     the very rows of ``x`` or of ``residual`` (in place), other overlaps are refused.
     """
     try:
-        key = (_sig(x, residual, weight), None if post_weight is None else _sig(post_weight), None if gate is None else _sig(gate),
-               None if residual_out is None else _sig(residual_out), None if out is None else _sig(out))
+        # one flat key: what the checks look at (the launches are short, and nested tuples cost as much as the checks)
+        key = (x.shape, x.stride(), x.dtype, x.device, residual.shape, residual.stride(), residual.dtype, residual.device, weight.shape,
+               weight.stride(), weight.dtype, weight.device,
+               None if post_weight is None else (post_weight.shape, post_weight.stride(), post_weight.dtype, post_weight.device),
+               None if gate is None else (gate.shape, gate.stride(), gate.dtype, gate.device),
+               None if residual_out is None else (residual_out.shape, residual_out.stride(), residual_out.dtype, residual_out.device),
+               None if out is None else (out.shape, out.stride(), out.dtype, out.device))
     except AttributeError:
         raise RuntimeError("residual_norms takes tensors") from None
     plan = _plans.get(key)
@@ -86,13 +93,17 @@ def residual_norms(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if args[0] == 0:
         return residual_out, out
-    px, pr, po, ph, pg = x.data_ptr(), residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(), None if gate is None else gate.data_ptr()
+    px, pr, po, ph, pg = x.data_ptr(), residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(), 0 if gate is None else gate.data_ptr()
     if given:
         # a row's values are all read before its outputs are written: an output may be the very rows of x or of the residual
-        _require(((po == px and so == sx) or _apart(po, *so, px, *sx, row)) and ((po == pr and so == sr) or _apart(po, *so, pr, *sr, row))
-                 and ((ph == px and sh == sx) or _apart(ph, *sh, px, *sx, row)) and ((ph == pr and sh == sr) or _apart(ph, *sh, pr, *sr, row))
-                 and _apart(po, *so, ph, *sh, row) and (pg is None or (_apart(po, *so, pg, *sg, row) and _apart(ph, *sh, pg, *sg, row))),
-                 "residual_norms: an output overlaps another tensor without being the same rows of x or residual")
-    _call(dev_index, _C.npd_residual_norms, po, ph, px, pr, weight.data_ptr(), None if post_weight is None else post_weight.data_ptr(), pg,
-          residual_scale, eps, weight_offset, *args, _raw_stream(dev_index))
+        (ex, tx), (er, tr), (eo, to), (eh, th) = sx, sr, so, sh
+        if not ((po + eo <= px or px + ex <= po or (po == px and to == tx) or _apart(po, eo, to, px, ex, tx, row))
+                and (po + eo <= pr or pr + er <= po or (po == pr and to == tr) or _apart(po, eo, to, pr, er, tr, row))
+                and (ph + eh <= px or px + ex <= ph or (ph == px and th == tx) or _apart(ph, eh, th, px, ex, tx, row))
+                and (ph + eh <= pr or pr + er <= ph or (ph == pr and th == tr) or _apart(ph, eh, th, pr, er, tr, row))
+                and (po + eo <= ph or ph + eh <= po or _apart(po, eo, to, ph, eh, th, row))
+                and (pg == 0 or (_apart(po, eo, to, pg, *sg, row) and _apart(ph, eh, th, pg, *sg, row)))):
+            raise RuntimeError("residual_norms: an output overlaps another tensor without being the same rows of x or residual")
+    _packed_op(NPD_OP_RESIDUAL_NORMS, _pack, dev_index, po, ph, px, pr, weight.data_ptr(), 0 if post_weight is None else post_weight.data_ptr(),
+               pg, residual_scale, eps, weight_offset, *args, _raw_stream(dev_index))
     return residual_out, out

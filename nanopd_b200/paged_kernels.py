@@ -15,7 +15,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 import threading
+from array import array
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -173,14 +175,33 @@ def _ws_ptr(dev_index: int, handle: int, nbytes: int):
 # status bits of all of them go to one word per device, which lives as long as the process.
 # ---------------------------------------------------------------------------
 _scratch: Dict[Tuple[int, int], torch.Tensor] = {}
+_packed_call = _C.npd_call_packed
+_pack_scored = struct.Struct("<q6Q2dQ11qQqQqQ").pack           # device, then the entry point's arguments
+_pack_scored_prefill = struct.Struct("<q8Qq2dQ10qQqQqQ").pack
+_pack_shared = struct.Struct("<q8Qd11qQqQqQ").pack
+
+
+def _packed_op(op: int, pack, *args) -> None:
+    """An operator's entry point, its arguments packed (see npd_call_packed)."""
+    try:
+        slots = pack(*args)
+    except struct.error:
+        raise RuntimeError("a number was expected") from None
+    rc = _packed_call(op, slots)
+    if rc:
+        _lib.check(rc)
+
+
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 _captured_scratch: Dict[Tuple[int, int], Tuple[int, torch.Tensor, int]] = {}     # the stream's latest capture; bytes cleared
 _status_words: Dict[int, torch.Tensor] = {}
+_status_addresses: Dict[int, int] = {}
 
 
 def _status_ptr(dev_index: int) -> int:
-    word = _status_words.get(dev_index)
-    if word is None:
-        _require(not torch.cuda.is_current_stream_capturing(),
+    address = _status_addresses.get(dev_index)
+    if address is None:
+        _require(not _capturing(),
                  "call the operator once on this device before capturing it (it allocates its status word on first use)")
         with _ws_lock:
             word = _status_words.get(dev_index)
@@ -188,14 +209,15 @@ def _status_ptr(dev_index: int) -> int:
                 made = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", dev_index))
                 torch.cuda.synchronize(dev_index)            # other streams may write it from now on
                 _status_words[dev_index] = word = made
-    return word.data_ptr()
+        address = _status_addresses[dev_index] = word.data_ptr()
+    return address
 
 
 def _scratch_for(dev_index: int, handle: int, nbytes: int, cleared: int) -> torch.Tensor:
     """At least ``nbytes`` of scratch for a call on the current stream (``handle``), the first ``cleared`` bytes zero when
     it is first used."""
     key = (dev_index, handle)
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         capture = ctypes.c_uint64(0)
         _lib.check(_C.npd_capture_id(handle, ctypes.byref(capture)))
         held = _captured_scratch.get(key)
@@ -583,7 +605,11 @@ def paged_scored_attention(out, query, key_cache, value_cache, block_tables, seq
     those of :func:`paged_attention_forward` (the interleaved layouts are not taken).
     """
     try:
-        key = (_sig(out, query, key_cache, value_cache, block_tables, seq_lens), block_size, max_num_blocks_per_seq,
+        # one flat key: what the checks look at (the calls are small, and nested tuples cost as much as the checks)
+        key = (out.shape, out.stride(), out.dtype, out.device, query.shape, query.stride(), query.dtype, query.device,
+               key_cache.shape, key_cache.stride(), key_cache.dtype, key_cache.device, value_cache.shape, value_cache.stride(),
+               value_cache.dtype, value_cache.device, block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device,
+               seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, block_size, max_num_blocks_per_seq,
                None if distance_slopes is None else _sig(distance_slopes), score_cap, window, max_ctas)
         plan = _scored_plans.get(key)
     except (AttributeError, TypeError):
@@ -596,15 +622,16 @@ def paged_scored_attention(out, query, key_cache, value_cache, block_tables, seq
         if S == 0:
             return
         need = _C.npd_decode_workspace_bytes(S, hq, hkv, d, dev.index)
-        plan = (dev.index, need, 256 + 4 * S * hq, int(max_ctas) << 8, float(score_cap), int(window),
+        plan = (dev.index, need, min(256 + 4 * S * hq, need), int(max_ctas) << 8, float(score_cap), int(window),
                 (S, hq, hkv, d, bs, max_blk, nb, cstride, row_stride, _DTYPE_CODE[query.dtype]))
         _remember(_scored_plans, key, plan)
     dev_index, need, cleared, flags, cap, win, args = plan
     handle = _raw_stream(dev_index)
-    ws = _scratch_for(dev_index, handle, need, min(cleared, need))
-    _call(dev_index, _C.npd_paged_scored_attention, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-          block_tables.data_ptr(), seq_lens.data_ptr(), float(scale), cap, None if distance_slopes is None else distance_slopes.data_ptr(), win,
-          *args, ws.data_ptr(), ws.numel(), _status_ptr(dev_index), flags, handle)
+    ws = _scratch_for(dev_index, handle, need, cleared)
+    _packed_op(_lib.NPD_OP_SCORED_ATTENTION, _pack_scored,
+        dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+        scale, cap, 0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws.data_ptr(), ws.numel(),
+        _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
@@ -627,8 +654,12 @@ def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tabl
     :func:`paged_attention_forward` (the interleaved layouts are not taken).
     """
     try:
-        key = (_sig(out, query, key_cache, value_cache, block_tables, seq_lens, group_offsets, shared_lens), block_size,
-               max_num_blocks_per_seq, max_ctas)
+        key = (out.shape, out.stride(), out.dtype, out.device, query.shape, query.stride(), query.dtype, query.device,
+               key_cache.shape, key_cache.stride(), key_cache.dtype, key_cache.device, value_cache.shape, value_cache.stride(),
+               value_cache.dtype, value_cache.device, block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device,
+               seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, group_offsets.shape, group_offsets.stride(),
+               group_offsets.dtype, group_offsets.device, shared_lens.shape, shared_lens.stride(), shared_lens.dtype, shared_lens.device,
+               block_size, max_num_blocks_per_seq, max_ctas)
         plan = _shared_plans.get(key)
     except (AttributeError, TypeError):
         raise RuntimeError("paged_shared_prefix_attention takes tensors and numbers") from None
@@ -646,15 +677,15 @@ def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tabl
         if S == 0:
             return
         need = _C.npd_shared_prefix_workspace_bytes(S, groups, hq, hkv, d, dev.index)
-        plan = (dev.index, need, 256 + 4 * S * hq, int(max_ctas) << 8,
+        plan = (dev.index, need, min(256 + 4 * S * hq, need), int(max_ctas) << 8,
                 (S, groups, hq, hkv, d, bs, max_blk, nb, cstride, row_stride, _DTYPE_CODE[query.dtype]))
         _remember(_shared_plans, key, plan)
     dev_index, need, cleared, flags, args = plan
     handle = _raw_stream(dev_index)
-    ws = _scratch_for(dev_index, handle, need, min(cleared, need))
-    _call(dev_index, _C.npd_paged_shared_prefix_attention, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-          block_tables.data_ptr(), seq_lens.data_ptr(), group_offsets.data_ptr(), shared_lens.data_ptr(), float(scale), *args,
-          ws.data_ptr(), ws.numel(), _status_ptr(dev_index), flags, handle)
+    ws = _scratch_for(dev_index, handle, need, cleared)
+    _packed_op(_lib.NPD_OP_SHARED_PREFIX_ATTENTION, _pack_shared,
+        dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+        group_offsets.data_ptr(), shared_lens.data_ptr(), scale, *args, ws.data_ptr(), ws.numel(), _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
@@ -677,7 +708,8 @@ def paged_scored_prefill_attention(out, query, key_cache, value_cache, block_tab
         dev = query.device
         total, hq, d = query.shape
         nchunks = len(chunk_tokens)
-        _require(len(chunk_q_offsets) == nchunks and len(chunk_starts) == nchunks and block_tables.size(0) == nchunks,
+        offs, toks, starts = array("i", chunk_q_offsets), array("i", chunk_tokens), array("i", chunk_starts)
+        _require(len(offs) == nchunks and len(starts) == nchunks and block_tables.size(0) == nchunks,
                  f"{name}: one offset, token count, start position and table row per chunk")
         _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and query.is_contiguous() and out.is_contiguous(),
                  f"{name}: out must match query in shape, dtype and device; both contiguous")
@@ -692,21 +724,20 @@ def paged_scored_prefill_attention(out, query, key_cache, value_cache, block_tab
         _require(1 <= max_blk <= block_tables.size(1), "max_num_blocks_per_seq out of range")
         _require(0 <= int(max_ctas) <= 0xffff, "max_ctas out of range")
         _score_shape(name, score_cap, distance_slopes, window, hq, dev)
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, OverflowError):
         raise RuntimeError(f"{name} takes tensors, lists of whole numbers and numbers") from None
-    for off, n, start in zip(chunk_q_offsets, chunk_tokens, chunk_starts):
+    for off, n, start in zip(offs, toks, starts):
         _require(n >= 0 and off >= 0 and off + n <= total and start >= 0, f"{name}: chunk outside the query tensor")
         _require(start + n <= max_blk * bs, f"{name}: chunk reaches beyond its block table")
     if nchunks == 0 or total == 0:
         return
-    arr = ctypes.c_int32 * nchunks
     handle = _raw_stream(dev.index)
-    need = _C.npd_prefill_workspace_bytes(total, hq, hkv, d, dev.index)
-    ws = _scratch_for(dev.index, handle, need, 256)
-    _call(dev.index, _C.npd_paged_scored_prefill_attention, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-          block_tables.data_ptr(), arr(*chunk_q_offsets), arr(*chunk_tokens), arr(*chunk_starts), nchunks, float(scale), float(score_cap),
-          None if distance_slopes is None else distance_slopes.data_ptr(), int(window), hq, hkv, d, bs, max_blk, nb, cstride,
-          block_tables.stride(0), _DTYPE_CODE[query.dtype], ws.data_ptr(), ws.numel(), _status_ptr(dev.index), int(max_ctas) << 8, handle)
+    ws = _scratch_for(dev.index, handle, 256, 256)
+    _packed_op(_lib.NPD_OP_SCORED_PREFILL_ATTENTION, _pack_scored_prefill,
+        dev.index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+        offs.buffer_info()[0], toks.buffer_info()[0], starts.buffer_info()[0], nchunks, scale, score_cap,
+        0 if distance_slopes is None else distance_slopes.data_ptr(), int(window), hq, hkv, d, bs, max_blk, nb, cstride, block_tables.stride(0),
+        _DTYPE_CODE[query.dtype], ws.data_ptr(), ws.numel(), _status_ptr(dev.index), int(max_ctas) << 8, handle)
 
 
 # ---------------------------------------------------------------------------

@@ -91,13 +91,15 @@ def test_empty_batch_and_empty_sequences(kernels):
     kernels.paged_scored_attention(q[:0], q[:0], kc, vc, bt[:0], sl[:0], scale, 16, bt.size(1), score_cap=30.0)
 
 
-def test_without_shaping_equals_the_plain_operator(kernels):
-    """Cap 0, no slopes, no window: the same scores, so the same row up to the order of sums."""
+def test_without_shaping_agrees_with_the_plain_operator(kernels):
+    """Cap 0, no slopes, no window: the same scores.  The two split a sequence at other places, so their sums differ in order:
+    each is within the tolerance of the 64-bit form, and within twice that of the other."""
     q, kc, vc, bt, sl, scale = make([700, 33, 1999, 16], 32, 8, 128, 16, torch.bfloat16)
-    out, plain = torch.empty_like(q), torch.empty_like(q)
-    kernels.paged_scored_attention(out, q, kc, vc, bt, sl, scale, 16, bt.size(1))
+    out, plain = check(kernels, q, kc, vc, bt, sl, scale), torch.empty_like(q)
     kernels.paged_attention_forward(plain, q, kc, vc, bt, sl, scale, 16, bt.size(1))
-    assert torch.equal(out, plain)
+    want, A, l = shaped_oracle.attend_single(q, kc, vc, bt, sl, scale)
+    tol = shaped_oracle.attention_tolerance(want, A, l, 1999, q.dtype, float(vc.abs().max()))
+    assert ((out.double() - plain.double()).abs() <= 2 * tol).all()
 
 
 def test_scores_far_beyond_the_cap(kernels):
