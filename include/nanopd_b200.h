@@ -289,7 +289,7 @@ int npd_paged_scored_prefill_attention(void *out, const void *q, const void *k_c
  * shared; the rest of a prefix is read per sequence.  The lengths, offsets and tables are read on
  * the device: they may change between replays of a captured call.  Offsets that are not
  * ascending within [0, num_seqs] and negative shared_lens raise NPD_STATUS_BAD_POSITION and
- * share nothing.  num_groups between 1 and 4096, num_q_heads/num_kv_heads <= 128; other shapes
+ * share nothing.  Small batches are answered by one launch without sharing.  num_groups between 1 and 4096, num_q_heads/num_kv_heads <= 128; other shapes
  * as in (2), without the interleaved layouts; `status` and `flags` as in (7).  `workspace`:
  * npd_shared_prefix_workspace_bytes(...) bytes, 256-byte aligned, zeroed once; two calls that may
  * overlap on the GPU need two workspaces.                                                   */

@@ -75,6 +75,9 @@ struct DecodeParams {
     float cap_log2;       // cap * log2(e)
     const float *slopes;  // [num_q_heads] slope of the distance bias, or nullptr
     int window;           // keys visible behind the query, its own included; INT32_MAX = all
+    int cluster;          // small form: CTAs that share a (sequence, virtual kv head)
+    const int32_t *group_offsets, *shared_lens;    // of a shared-prefix call that shares nothing, or nullptr
+    int num_groups;
     // kTail: what the prefix pass left (see shared_prefix.cu)
     const PrefixSeqPlan *seq_plan;   // [num_seqs]
     int seq_base;                           // index of the launch's first sequence in the call's batch
@@ -387,6 +390,83 @@ __device__ __forceinline__ void merge_records(AttnState<T, D, NT> &st, const flo
     }
 }
 
+// ---- the merge of the small form in a cluster of CTAs (kScored) ----
+// One 16-element slice (nt, j) of a merged record: this lane's four values and the maxima and sums of its two heads.
+template <int D, int NT>
+struct SliceSum {
+    float4 o;
+    float m0, m1, l0, l1;
+};
+// A record in the shared memory of CTA `rank` of the cluster, at the same address as in this CTA.
+struct RemoteFloats {
+    uint32_t local, rank;
+    __device__ __forceinline__ float4 at(int index4) const {
+        uint32_t addr;
+        float4 v;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(local), "r"(rank));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(addr + static_cast<uint32_t>(index4) * 16u)
+                     : "memory");
+        return v;
+    }
+};
+__device__ __forceinline__ float4 record_at(const float *rec, int index4) { return reinterpret_cast<const float4 *>(rec)[index4]; }
+__device__ __forceinline__ float4 record_at(const RemoteFloats &rec, int index4) { return rec.at(index4); }
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Slice `sl` of `count` (at least one) records: the maximum over all of them first, then the weighted sum.
+template <int D, int NT, typename Record>
+__device__ __forceinline__ SliceSum<D, NT> merge_slice(int count, int sl, int lane, Record record) {
+    constexpr int KS = D / 16;
+    const int ml_at = NT * KS * 32 + sl / KS * 4 + (lane & 3);
+    SliceSum<D, NT> x{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f, 0.f};
+#pragma unroll 4
+    for (int w = 0; w < count; ++w) {
+        const float4 ml = record_at(record(w), ml_at);
+        x.m0 = fmaxf(x.m0, ml.x);
+        x.m1 = fmaxf(x.m1, ml.y);
+    }
+#pragma unroll 4
+    for (int w = 0; w < count; ++w) {
+        const float4 ml = record_at(record(w), ml_at), o = record_at(record(w), sl * 32 + lane);
+        const float s0 = fast_exp2(ml.x - x.m0), s1 = fast_exp2(ml.y - x.m1);        // maxima are finite in kScored
+        x.l0 += ml.z * s0;
+        x.l1 += ml.w * s1;
+        x.o.x += o.x * s0;
+        x.o.y += o.y * s1;
+        x.o.z += o.z * s0;
+        x.o.w += o.w * s1;
+    }
+    return x;
+}
+
+// Normalises a slice and writes its elements of the rows of (sequence, virtual kv head).
+template <typename T, int D, int NT>
+__device__ __forceinline__ void write_slice(const SliceSum<D, NT> &x, const DecodeParams &p, int s, int h, int sl, int lane) {
+    constexpr int KS = D / 16;
+    const int nt = sl / KS, j = sl - nt * KS, g = lane >> 2, t = lane & 3, head = nt * 8 + g;
+    const float inv0 = 1.f / x.l0, inv1 = 1.f / x.l1;
+    // (d = g, heads 2t..2t+1) -> transpose -> (head g, d = 2t..2t+1)
+    const uint32_t u0 = movmatrix_trans(Elem<T>::pack2(x.o.x * inv0, x.o.y * inv1));
+    const uint32_t u1 = movmatrix_trans(Elem<T>::pack2(x.o.z * inv0, x.o.w * inv1));
+    if (head < p.group) {
+        T *row = static_cast<T *>(p.out) + ((long long)s * p.num_q_heads + (long long)h * p.group + head) * D;
+        *reinterpret_cast<uint32_t *>(row + 16 * j + 2 * t) = u0;
+        *reinterpret_cast<uint32_t *>(row + 16 * j + 8 + 2 * t) = u1;
+    }
+}
+
+// A shared-prefix call that is answered without sharing (see shared_prefix.cu) still reports what its arguments have wrong.
+__device__ void check_groups(const DecodeParams &p) {
+    for (int i = threadIdx.x; i < p.num_groups; i += blockDim.x) {
+        const int a = __ldg(p.group_offsets + i), b = __ldg(p.group_offsets + i + 1);
+        if (a < 0 || b < a || b > p.num_seqs || __ldg(p.shared_lens + i) < 0) atomicOr(p.status, NPD_STATUS_BAD_POSITION);
+    }
+}
+
 // Folds the partial records of workers wf..wl (one (sequence, kv head) cut by range boundaries) into `st`.
 // Records were written by other SMs during this launch: read them through L2 (ld.global.cg), never L1.
 // Two passes, so that no load waits for arithmetic on an earlier one: first the maximum over all records (eight
@@ -633,7 +713,8 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
     uint8_t *stage_base = sbase + (size_t)warp * nst * STAGE_BYTES;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sbase + (size_t)nwarps * nst * STAGE_BYTES) + warp * nst;
     int *pre = reinterpret_cast<int *>(sbase + (size_t)nwarps * nst * (STAGE_BYTES + 8));
-    float *scratch = nullptr;        // kTail: this warp's rows on their way out
+    float *scratch = nullptr;        // kTail: this warp's rows on their way out; a cluster: the CTA's record
+    if (SMALL && MODE == kScored) scratch = reinterpret_cast<float *>(pre + 4);
     if (MODE == kTail)
         scratch = reinterpret_cast<float *>(pre + (p.num_seqs + 4) / 4 * 4) + warp * ((joined_floats(D, p.group) + 3) / 4 * 4);
 
@@ -649,25 +730,31 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
     long long W = 0;
     int worker = 0, my_tiles = 0;
     Cursor pc, cc;                   // producer / consumer cursors over the same range
+    constexpr bool CLUSTER = SMALL && MODE == kScored;       // a (sequence, kv head) belongs to a cluster of CTAs
+    const int cta_rank = CLUSTER ? static_cast<int>(blockIdx.x) % p.cluster : 0;
     if (SMALL) {
         __syncthreads();             // barriers are initialised for everyone
-        const int s0 = blockIdx.x / p.num_vheads, h0 = blockIdx.x - s0 * p.num_vheads;
+        const int pair = CLUSTER ? static_cast<int>(blockIdx.x) / p.cluster : static_cast<int>(blockIdx.x);
+        const int s0 = pair / p.num_vheads, h0 = pair - s0 * p.num_vheads;
         const int raw = __ldg(p.seq_lens + s0);
-        if ((raw < 0 || raw > (long long)p.max_blocks_per_seq * p.block_size) && h0 == 0 && threadIdx.x == 0)
+        if ((raw < 0 || raw > (long long)p.max_blocks_per_seq * p.block_size) && h0 == 0 && cta_rank == 0 && threadIdx.x == 0)
             atomicOr(p.status, NPD_STATUS_BAD_POSITION);
+        if (CLUSTER && p.group_offsets != nullptr && blockIdx.x == 0) check_groups(p);
         const int len0 = clamped_len(p, s0), first0 = first_tile<MODE>(p, s0, len0);
         const int n0 = (len0 + kTile - 1) / kTile - first0;
         if (n0 == 0) {
             // an empty sequence gets zero rows (see below); this CTA writes those of its own q heads
             uint32_t *row = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) +
                                                          ((long long)s0 * p.num_q_heads + (long long)h0 * p.group) * D);
-            for (int i = threadIdx.x; i < p.group * D / 2; i += blockDim.x) row[i] = 0u;
-            return;                  // the whole CTA leaves here: no barrier follows for anyone
+            if (cta_rank == 0)
+                for (int i = threadIdx.x; i < p.group * D / 2; i += blockDim.x) row[i] = 0u;
+            return;                  // the whole CTA (and cluster) leaves here: no barrier follows for anyone
         }
-        const int per_warp = (n0 + nwarps - 1) / nwarps;
-        const int t0 = warp * per_warp;
+        const int workers = CLUSTER ? nwarps * p.cluster : nwarps;
+        const int per_warp = (n0 + workers - 1) / workers;
+        worker = cta_rank * nwarps + warp;
+        const int t0 = worker * per_warp;
         W = per_warp;
-        worker = warp;
         my_tiles = max(0, min(per_warp, n0 - t0));
         pc.s = s0, pc.h = h0, pc.t = min(t0, n0 - 1), pc.n = n0, pc.len = len0, pc.first = first0;
     } else {
@@ -984,7 +1071,39 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
         }
     }
 
-    if (SMALL) {
+    if constexpr (CLUSTER) {
+        // Two levels.  In each CTA the warps take the 16-element slices of the record between them and leave one record in
+        // `scratch`; then the slices are dealt out over the CTAs of the cluster, which read each other's records and write
+        // the rows' elements.  A slice is one float4 a lane and record, all of them under way at once.
+        __syncthreads();             // every warp's record is in shared memory (all warps of the CTA get here)
+        const int all = (pc.n + static_cast<int>(W) - 1) / static_cast<int>(W);      // warps of the cluster that had tiles
+        const int mine = max(0, min(nwarps, all - cta_rank * nwarps));
+        const size_t stride = (size_t)nst * STAGE_BYTES / sizeof(float);
+        const float *records = reinterpret_cast<const float *>(sbase);
+        constexpr int kSlices = NT * KS;
+        if (p.cluster == 1) {
+            for (int sl = warp; sl < kSlices; sl += nwarps) {
+                const SliceSum<D, NT> x = merge_slice<D, NT>(mine, sl, lane, [&](int w) { return records + w * stride; });
+                write_slice<T, D, NT>(x, p, pc.s, pc.h, sl, lane);
+            }
+        } else {
+            if (mine > 0)
+                for (int sl = warp; sl < kSlices; sl += nwarps) {
+                    const SliceSum<D, NT> x = merge_slice<D, NT>(mine, sl, lane, [&](int w) { return records + w * stride; });
+                    reinterpret_cast<float4 *>(scratch)[sl * 32 + lane] = x.o;
+                    if (sl % KS == 0 && g == 0)
+                        reinterpret_cast<float4 *>(scratch + kSlices * 128)[sl / KS * 4 + t4] = make_float4(x.m0, x.m1, x.l0, x.l1);
+                }
+            cluster_barrier();       // the CTAs' records are there
+            const int ctas = (all + nwarps - 1) / nwarps;        // of the cluster that had tiles
+            for (int sl = cta_rank + warp * p.cluster; sl < kSlices; sl += nwarps * p.cluster) {
+                const uint32_t local = smem_u32(scratch);
+                const SliceSum<D, NT> x = merge_slice<D, NT>(ctas, sl, lane, [&](int w) { return RemoteFloats{local, static_cast<uint32_t>(w)}; });
+                write_slice<T, D, NT>(x, p, pc.s, pc.h, sl, lane);
+            }
+            cluster_barrier();       // nobody leaves while its record may still be read
+        }
+    } else if (SMALL) {
         __syncthreads();             // every warp's record is in shared memory (all warps of the CTA get here)
         if (warp == 0) {
             const int n_records = (pc.n + static_cast<int>(W) - 1) / static_cast<int>(W);     // warps that had tiles
@@ -1014,6 +1133,7 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
 struct LaunchShape {
     int nwarps, nstages, grid;
     bool small;     // the small-batch form: one CTA per (sequence, virtual kv head)
+    int cluster = 1;      // kScored: that many CTAs per (sequence, virtual kv head)
 };
 
 int env_int(const char *name, int fallback) {
@@ -1033,7 +1153,7 @@ int env_int(const char *name, int fallback) {
 //   D=256:              4 warps x 3 stages 135, 8 warps x 1 stage 122
 //   D=128, one sequence of 8k / 64k tokens: 3 stages 29 / 76, 2 stages 36 / 86
 LaunchShape launch_shape(int head_dim, int block_size, int cta_cap, long long num_seq_heads, int device) {
-    LaunchShape ls;
+    LaunchShape ls{};
     const int stage_bytes = 2 * kTile * head_dim * 2;
     const int sms = npd::sm_count(device);
     // tuning knobs from the environment, read once per process
@@ -1075,6 +1195,28 @@ void consider_small_form(LaunchShape &ls, int head_dim, long long max_tokens, lo
     while (ls.nstages > 1 && (long long)ls.nwarps * ls.nstages * stage_bytes > 192 * 1024) --ls.nstages;
 }
 
+// kScored's small form: a cluster of CTAs to a (sequence, kv head), as many as leave every cluster a place (clusters of 8 of
+// these CTAs, one to an SM, fit 16 at a time), up to kClusterTokens tokens per CTA; beyond that the streaming form's equal
+// split wins.  Device time per launch, small form / streaming form (32/8 heads of 128, capped): 1 sequence of 256 tokens
+// 7.2 / 11.2 us, of 2048 10 / 19, of 8192 17.5 / 32, of 16000 32 / 43; 8 of 2000 18.6 / 27; 16 of 1000 17.6 / 24.6; 70 of 1000
+// (12/2 heads) 18.3 / 26.  Twelve warps to a CTA: 8 of 2000 20.4 us with eight.
+constexpr long long kClusterTokens = 2176;
+constexpr int kClusterWarps = 12;
+void consider_cluster_form(LaunchShape &ls, int head_dim, long long max_tokens, long long seq_heads, int cta_cap, int flags, int device) {
+    if ((flags & NPD_DECODE_NO_SMALL) || cta_cap > 0 || seq_heads < 1 || seq_heads > npd::sm_count(device)) return;
+    int cluster = seq_heads <= 16 ? 8 : (seq_heads <= 32 ? 4 : (seq_heads <= 64 ? 2 : 1));
+    if (max_tokens > kClusterTokens * cluster) return;
+    const int nwarps = head_dim == 256 ? 8 : kClusterWarps;
+    // a warp has a tile at least
+    while (cluster > 1 && (cluster / 2) * nwarps * kTile >= max_tokens) cluster /= 2;
+    const int stage_bytes = 2 * kTile * head_dim * 2;
+    ls.small = true;
+    ls.cluster = cluster;
+    ls.grid = static_cast<int>(seq_heads) * cluster;
+    ls.nwarps = nwarps;
+    ls.nstages = head_dim == 256 ? 1 : (head_dim == 128 ? 3 : 4);
+    while (ls.nstages > 1 && (long long)ls.nwarps * ls.nstages * stage_bytes > 192 * 1024) --ls.nstages;
+}
 // Smallest split of the group into virtual kv heads whose q-head count fits the n-tiles.
 int choose_kv_rep(int group, int max_heads) {
     for (int r = 1; r <= group; ++r)
@@ -1095,7 +1237,9 @@ template <int MODE, typename T, int D, int NT, bool IL>
 int launch_decode(const DecodeParams &p, const CUtensorMap &tk, const CUtensorMap &tv, const LaunchShape &ls,
                   cudaStream_t stream) {
     constexpr int STAGE_BYTES = 2 * kTile * D * 2;
-    const size_t smem = MODE == kTail ? tail_smem(D, p.group, ls, p.num_seqs)
+    // (the small form needs no prefix over the sequences)
+    const size_t smem = MODE == kScored && ls.small ? 1024 + (size_t)ls.nwarps * ls.nstages * (STAGE_BYTES + 8) + 32 :
+                        MODE == kTail ? tail_smem(D, p.group, ls, p.num_seqs)
                                       : 1024 + (size_t)ls.nwarps * ls.nstages * (STAGE_BYTES + 8) + ((size_t)p.num_seqs + 1) * 4 + 16;
     if constexpr (MODE == kTail) {
         // launched while the prefix pass still runs; waits for it before it reads anything that it or the plan wrote
@@ -1132,12 +1276,22 @@ int launch_decode(const DecodeParams &p, const CUtensorMap &tk, const CUtensorMa
                 NPD_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
                 npd::set_up_on_device(done, dev);
             }
-            kern<<<ls.grid, ls.nwarps * 32, smem, stream>>>(p, tk, tv);
-            NPD_CUDA_TRY(cudaGetLastError());
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(ls.grid);
+            cfg.blockDim = dim3(ls.nwarps * 32);
+            cfg.dynamicSmemBytes = smem + (ls.small ? rec_floats<D, NT>() * sizeof(float) : 0);
+            cfg.stream = stream;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = ls.cluster;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = ls.cluster > 1 ? 1 : 0;
+            NPD_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, tk, tv));
             return NPD_OK;
         };
         static std::atomic<unsigned long long> done_small{0}, done8{0}, done12{0};
-        if (ls.small) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, true, MODE>, done_small);
+        if (ls.small) return launch(paged_decode_stream_kernel<T, D, NT, IL, kClusterWarps, true, MODE>, done_small);
         if (ls.nwarps <= 8) return launch(paged_decode_stream_kernel<T, D, NT, IL, 8, false, MODE>, done8);
         return launch(paged_decode_stream_kernel<T, D, NT, IL, NPD_DECODE_MAX_WARPS, false, MODE>, done12);
     } else {
@@ -1217,6 +1371,8 @@ struct DecodeCall {
     float score_cap = 0.f;
     const float *slopes = nullptr;
     int64_t window = 0;              // 0: no window
+    const int32_t *group_offsets = nullptr, *shared_lens = nullptr;     // looked at by the small form only, see check_groups
+    int64_t num_groups = 0;
     // kTail
     const PrefixSeqPlan *seq_plan = nullptr;
     const PrefixPlanHead *plan_head = nullptr;
@@ -1248,6 +1404,17 @@ inline int check_decode_call(const DecodeCall &c) {
     return NPD_OK;
 }
 
+// Whether run_decode<kScored> takes its small form for this call.
+inline bool takes_cluster_form(const DecodeCall &c) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    LaunchShape ls{};
+    const WorkspacePlan wp = plan_workspace(c.num_seqs, c.num_q_heads, c.num_kv_heads, c.head_dim, ls);
+    consider_cluster_form(ls, static_cast<int>(c.head_dim), (long long)c.max_blocks_per_seq * c.block_size,
+                          (long long)c.num_seqs * c.num_kv_heads * wp.kv_rep, (c.flags >> 8) & 0xffff, c.flags, dev);
+    return ls.small;
+}
+
 template <int MODE>
 int run_decode(const DecodeCall &c) {
     int dev = 0;
@@ -1263,7 +1430,10 @@ int run_decode(const DecodeCall &c) {
     // the longest run of keys a sequence can have: the table's width bounds it, and so does a window
     long long max_tokens = (long long)c.max_blocks_per_seq * c.block_size;
     if (MODE == kScored && c.window > 0 && c.window + kTile < max_tokens) max_tokens = c.window + kTile;
-    if (MODE != kTail)
+    if (MODE == kScored)
+        consider_cluster_form(ls, static_cast<int>(c.head_dim), max_tokens, (long long)c.num_seqs * c.num_kv_heads * wp.kv_rep,
+                              (c.flags >> 8) & 0xffff, c.flags, dev);
+    else if (MODE == kPlain)
         consider_small_form(ls, static_cast<int>(c.head_dim), max_tokens,
                         (long long)c.num_seqs * c.num_kv_heads * wp.kv_rep, (c.flags >> 8) & 0xffff,
                         (c.flags & NPD_DECODE_KV_INTERLEAVED) != 0, c.flags, dev);
@@ -1327,6 +1497,10 @@ int run_decode(const DecodeCall &c) {
     p.slopes = c.slopes;
     p.window = c.window > 0 && c.window < INT32_MAX ? static_cast<int>(c.window) : INT32_MAX;
     p.seg_cost = MODE == kTail ? 6 : 2;
+    p.cluster = ls.cluster;
+    p.group_offsets = c.group_offsets;
+    p.shared_lens = c.shared_lens;
+    p.num_groups = static_cast<int>(c.num_groups);
     p.plan_head = c.plan_head;
     p.prefix_o = c.prefix_o;
     p.prefix_lse = c.prefix_lse;

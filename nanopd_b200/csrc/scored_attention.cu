@@ -27,3 +27,15 @@ extern "C" int npd_paged_scored_attention(void *out, const void *q, const void *
     const int rc = check_decode_call(c);
     return rc != NPD_OK || num_seqs == 0 ? rc : run_decode<kScored>(c);
 }
+
+int npd::decode_unshared_if_small(const npd::SharedCall &a, bool *taken) {
+    DecodeCall c{a.out, a.q, a.k_cache, a.v_cache, a.block_tables, a.seq_lens, a.scale, a.num_seqs, a.num_q_heads, a.num_kv_heads,
+                 a.head_dim, a.block_size, a.max_blocks_per_seq, a.num_blocks, a.cache_block_stride, a.bt_row_stride, a.dtype,
+                 a.workspace, a.workspace_bytes, a.flags, a.stream};
+    c.status = a.status;
+    c.group_offsets = a.group_offsets;
+    c.shared_lens = a.shared_lens;
+    c.num_groups = a.num_groups;
+    *taken = takes_cluster_form(c);
+    return *taken ? run_decode<kScored>(c) : NPD_OK;
+}

@@ -229,6 +229,17 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
                 "shared-prefix attention: batch times context exceeds int32");
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     if (status == nullptr) status = reinterpret_cast<int32_t *>(ws);
+    {
+        // A small batch whose sequences fit a cluster of CTAs each is answered by that one launch: reading the shared pages
+        // again (they are in L2) costs less than three launches.  16 sequences behind 992 shared tokens, 12/2 heads:
+        // 9.6 us, with sharing 29 us.
+        const npd::SharedCall sc{out, q, k_cache, v_cache, block_tables, seq_lens, group_offsets, shared_lens, scale, num_seqs, num_groups,
+                                 num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks, cache_block_stride,
+                                 bt_row_stride, dtype, workspace, decode_bytes, status, flags, stream};
+        bool taken = false;
+        rc = npd::decode_unshared_if_small(sc, &taken);
+        if (taken || rc != NPD_OK) return rc;
+    }
     PlanParams pp;
     pp.group_offsets = group_offsets;
     pp.shared_lens = shared_lens;

@@ -54,4 +54,22 @@ struct PrefixPass {
 };
 int launch_prefix_pass(const PrefixPass &a);
 
+// A shared-prefix call (scored_attention.cu): answered without sharing, by the small form of the decode kernel, where that
+// form takes the batch; *taken says whether it did.
+struct SharedCall {
+    void *out;
+    const void *q, *k_cache, *v_cache;
+    const int32_t *block_tables, *seq_lens, *group_offsets, *shared_lens;
+    float scale;
+    int64_t num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks,
+        cache_block_stride, bt_row_stride;
+    int dtype;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t *status;
+    int flags;
+    void *stream;
+};
+int decode_unshared_if_small(const SharedCall &a, bool *taken);
+
 }  // namespace npd
