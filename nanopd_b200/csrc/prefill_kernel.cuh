@@ -968,10 +968,11 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
             const ItemT it = ctrl->sched_desc[k % kSchedSlots];
-            const int U = it.nhalf[x];
+            const int U = x == 0 ? it.nhalf[0] : it.nhalf[1];
             const int t0 = item_t0<MODE>(it);
+            const int first_pos = it.start + (x == 0 ? it.tok0[0] : it.tok0[1]);       // of the tile's first row
             // last visible key of this row
-            const int pos = MODE == kPrefix ? it.ctx_end - 1 : it.start + it.tok0[x] + tq_idx;
+            const int pos = MODE == kPrefix ? it.ctx_end - 1 : first_pos + tq_idx;
             float slope2 = 0.f;                                  // kShaped: slope of this row's head, log2 domain
             if constexpr (shapes(MODE))
                 if (p.slopes != nullptr && row < p.tq * p.group) slope2 = __ldg(p.slopes + it.h * p.group + hg) * 1.4426950408889634f;
@@ -1015,56 +1016,21 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 for (int cc = 0; cc < 2; ++cc) tmem_ld32(t_sx + buf * kHalfKeys + cc * 32, sc[cc]);
                 tmem_wait_ld();
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 22, u);
-                const int first_pos = it.start + it.tok0[x];       // of the tile's first row
                 const bool diagonal = key0 + kHalfKeys - 1 > first_pos;      // reaches past the first row's diagonal
-                float m_new, bias0 = 0.f;    // bias0: the distance bias of the half-step's first key
-                bool direct = false;         // kCapped: the scores are still raw, their cap is a polynomial
-                if constexpr (shapes(MODE)) {
-                    const bool behind = key0 <= first_pos + p.tq - 1 - p.window;     // begins before the last row's window
-                    if (MODE == kCapped && !diagonal && !behind && p.slopes == nullptr) {
-                        // tanh grows with its argument: the largest capped score is that of the largest raw one
-                        const float mx = row_max(sc);
-                        direct = !__any_sync(0xffffffffu, fmaxf(mx, -row_min(sc)) >= p.cap_reach);
-                        if (direct) m_new = mx * cap_factor2(make_float2(mx * mx, 0.f), p).x;
+                const bool behind = shapes(MODE) && key0 <= first_pos + p.tq - 1 - p.window;     // begins before the last row's window
+                // Lazy correction: O (in TMEM) and l are rescaled only when some row's maximum grew by more than 2^8; otherwise
+                // the stale maximum keeps every probability below 256, exactly cancelled by the final division.  O may be
+                // touched once every PV product issued so far has completed: PV(u-1) is the last one (PV(u) waits for the
+                // probabilities of this half-step); the one before it on the same barrier, PV(u-3), is known to be complete
+                // (s_full of this buffer covers PV(u-2)).
+                auto new_maximum = [&](float m_new) {
+                    if (u == 0) {
+                        m_run = m_new;                              // kCausal: key 0 is visible to every row, so it is finite
+                        return true;
                     }
-                    if (!direct) {
-                        if (MODE == kCapped || p.slopes != nullptr) bias0 = shape_scores<MODE == kCapped>(sc, slope2, key0 - pos, p);
-                        if (diagonal || behind) {
-                            const int before = pos - p.window;           // last key that is out of this row's window
-#pragma unroll
-                            for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const int key = key0 + cc * 32 + i;
-                                    if (key > pos || key <= before) sc[cc][i] = -INFINITY;
-                                }
-                        }
-                        // a half-step that a row sees nothing of (or scores of -inf): any finite maximum serves
-                        m_new = fmaxf(row_max(sc) * (MODE == kShaped && p.slopes == nullptr ? p.scale_log2 : 1.f) + bias0, -3.0e38f);
-                    }
-                } else {
-                    // kPrefix: only keys behind the piece are masked
-                    if (MODE == kPrefix ? key0 + kHalfKeys > it.ctx_end : diagonal) {
-#pragma unroll
-                        for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
-                    }
-                    m_new = row_max(sc) * p.scale_log2;
-                }
-                if (u == 0) {
-                    m_run = m_new;                              // key 0 is visible to every row: finite
-                } else {
-                    // Lazy correction: O (in TMEM) and l are rescaled only when some row's maximum grew by more
-                    // than 2^8; otherwise the stale maximum keeps every probability below 256, exactly cancelled
-                    // by the final division.  O may be touched once every PV product issued so far has completed:
-                    // PV(u-1) is the last one (PV(u) waits for the probabilities of this half-step); the one before
-                    // it on the same barrier, PV(u-3), is known to be complete (s_full of this buffer covers PV(u-2)).
                     const bool grow = m_new > m_run + kRescaleThreshold;
                     if (__any_sync(0xffffffffu, grow)) {
-                        if (!(ok = wait_or_abort(smem_u32(&ctrl->pv_done[x][(cu - 1) & 1]), ((cu - 1) >> 1) & 1, abort_flag,
-                                                 p.status))) break;
+                        if (!wait_or_abort(smem_u32(&ctrl->pv_done[x][(cu - 1) & 1]), ((cu - 1) >> 1) & 1, abort_flag, p.status)) return false;
                         tc_fence_after();
                         const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
 #pragma unroll 1
@@ -1082,42 +1048,93 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                             m_run = m_new;
                         }
                     }
-                }
-                if (lane == 0) NPD_TRACE_FINE(sm_role, 23, u);
-                // ---- probabilities (masked scores are -inf -> 0), packed in pairs over the first 32 columns of the
-                //      buffer just read ----
-                const float scale1 = MODE == kShaped && p.slopes != nullptr ? 1.f : p.scale_log2;
-                const float2 scale2 = make_float2(scale1, scale1);
-                const float negm = shapes(MODE) ? bias0 - m_run : -m_run;
-                const float2 negm2 = make_float2(negm, negm);
-                if constexpr (MODE == kCapped) {
+                    return true;
+                };
+                // Probabilities (masked scores are -inf -> 0) from the pairs' exponents, packed over the first 32 columns of the
+                // buffer just read.
+                auto probabilities = [&](auto exponents) {
+                    float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int cc = 0; cc < 2; ++cc)
+                    for (int cc = 0; cc < 2; ++cc) {
+                        uint32_t packed[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            float2 y = make_float2(sc[cc][i], sc[cc][i + 1]);
-                            y = direct ? __ffma2_rn(cap_factor2(__fmul2_rn(y, y), p), y, negm2) : __fadd2_rn(y, negm2);
-                            sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 xs = exponents(make_float2(sc[cc][2 * i], sc[cc][2 * i + 1]));
+                            // a cap already fills the FMA pipes: all exponentials on the special-function unit
+                            // (chunks of 512 tokens: 363 us; a quarter of them on the FMA pipes 380, an eighth 368)
+                            constexpr int kEvery = MODE == kCapped ? 0 : kPolyExpEvery;
+                            const float2 pr = (kEvery > 0 && i % (kEvery > 0 ? kEvery : 1) == 0)
+                                                  ? exp2_fma2(xs)
+                                                  : make_float2(fast_exp2(xs.x), fast_exp2(xs.y));
+                            acc2[i & 1] = __fadd2_rn(acc2[i & 1], pr);
+                            packed[i] = Elem<T>::pack2(pr.x, pr.y);
                         }
-                }
-                float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    uint32_t packed[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 raw = make_float2(sc[cc][2 * i], sc[cc][2 * i + 1]);
-                        const float2 xs = MODE == kCapped ? raw : __ffma2_rn(raw, scale2, negm2);
-                        const float2 pr = (kPolyExpEvery > 0 && i % (kPolyExpEvery > 0 ? kPolyExpEvery : 1) == 0)
-                                              ? exp2_fma2(xs)
-                                              : make_float2(fast_exp2(xs.x), fast_exp2(xs.y));
-                        acc2[i & 1] = __fadd2_rn(acc2[i & 1], pr);
-                        packed[i] = Elem<T>::pack2(pr.x, pr.y);
+                        tmem_st16(t_sx + buf * kHalfKeys + cc * 16, packed);
                     }
-                    tmem_st16(t_sx + buf * kHalfKeys + cc * 16, packed);
+                    l_run += (acc2[0].x + acc2[1].x) + (acc2[0].y + acc2[1].y);
+                };
+                // Each way through a half-step goes from the raw scores to the stored probabilities on its own: where two of
+                // them meet with 64 scores in registers, the registers have to be moved to agree (35 instructions of 500).
+                if constexpr (shapes(MODE)) {
+                    auto mask = [&]() {
+                        if (!diagonal && !behind) return;
+                        const int before = pos - p.window;           // last key that is out of this row's window
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const int key = key0 + cc * 32 + i;
+                                if (key > pos || key <= before) sc[cc][i] = -INFINITY;
+                            }
+                    };
+                    // a half-step that a row sees nothing of (or scores of -inf): any finite maximum serves
+                    auto shaped = [&]() {
+                        const float bias0 = shape_scores<MODE == kCapped>(sc, slope2, key0 - pos, p);      // bias of the first key
+                        mask();
+                        if (!new_maximum(fmaxf(row_max(sc) + bias0, -3.0e38f))) return false;
+                        const float2 negm2 = make_float2(bias0 - m_run, bias0 - m_run);
+                        probabilities([&](float2 y) { return __fadd2_rn(y, negm2); });
+                        return true;
+                    };
+                    if (MODE == kCapped) {
+                        bool direct = !diagonal && !behind && p.slopes == nullptr;
+                        float mx = 0.f;
+                        if (direct) {
+                            // tanh grows with its argument: the largest capped score is that of the largest raw one
+                            mx = row_max(sc);
+                            direct = !__any_sync(0xffffffffu, fmaxf(mx, -row_min(sc)) >= p.cap_reach);
+                        }
+                        if (direct) {
+                            if (!(ok = new_maximum(mx * cap_factor2(make_float2(mx * mx, 0.f), p).x))) break;
+                            const float2 negm2 = make_float2(-m_run, -m_run);
+                            // the cap's polynomial in the same loop as the exponentials: the FMA and special-function pipes
+                            // work side by side (chunks of 512 tokens: 380 us, with two loops one after the other 395)
+                            probabilities([&](float2 y) { return __ffma2_rn(cap_factor2(__fmul2_rn(y, y), p), y, negm2); });
+                        } else if (!(ok = shaped())) {
+                            break;
+                        }
+                    } else if (p.slopes == nullptr) {
+                        mask();
+                        if (!(ok = new_maximum(fmaxf(row_max(sc) * p.scale_log2, -3.0e38f)))) break;
+                        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), negm2 = make_float2(-m_run, -m_run);
+                        probabilities([&](float2 y) { return __ffma2_rn(y, scale2, negm2); });
+                    } else if (!(ok = shaped())) {
+                        break;
+                    }
+                } else {
+                    // kPrefix: only keys behind the piece are masked
+                    if (MODE == kPrefix ? key0 + kHalfKeys > it.ctx_end : diagonal) {
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
+                    }
+                    if (!(ok = new_maximum(row_max(sc) * p.scale_log2))) break;
+                    if (lane == 0) NPD_TRACE_FINE(sm_role, 23, u);
+                    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), negm2 = make_float2(-m_run, -m_run);
+                    probabilities([&](float2 y) { return __ffma2_rn(y, scale2, negm2); });
                 }
-                const float psum = (acc2[0].x + acc2[1].x) + (acc2[0].y + acc2[1].y);
-                l_run += psum;
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 24, u);
                 if constexpr (shapes(MODE)) {
                     if (u == 0 && it.lo > key0) {                // V rows before the item's window may hold anything: clear them before PV reads them
@@ -1151,7 +1168,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                     !(ok = wait_or_abort(smem_u32(&ctrl->o_free[x]), (items_handed - 1) & 1, abort_flag, p.status))) break;
                 ctrl->l_sum[x][row] = l_run;
                 if constexpr (MODE == kPrefix) {
-                    if (tq_idx < it.tq_valid[x] && row < p.tq * p.group)
+                    if (tq_idx < (x == 0 ? it.tq_valid[0] : it.tq_valid[1]) && row < p.tq * p.group)
                         p.prefix_lse[(long long)it.row0 + (long long)blockIdx.x * kPrefixRows + (x * p.tq + tq_idx) * p.group + hg] =
                             m_run + log2f(l_run);
                 }
