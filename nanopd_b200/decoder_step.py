@@ -21,7 +21,7 @@ from typing import List, Optional
 import torch
 import torch.nn.functional as F
 
-from . import paged_kernels, sampling
+from . import norms, paged_kernels, sampling
 
 
 @dataclass
@@ -36,13 +36,26 @@ class DecoderShape:
     rope_theta: float = 1e6
     eps: float = 1e-6
     qk_norm: bool = True
+    # what some models of this family of shapes have besides; all off by default
+    score_cap: float = 0.0          # attention scores capped by score_cap * tanh(x / score_cap)
+    distance_bias: bool = False     # a bias linear in the distance to the key, slopes 2^(-8 (h + 1) / num_q_heads)
+    window: int = 0                 # keys that a layer with a sliding window sees
+    window_every: int = 1           # layer i has the window when i is a multiple of this, the others see everything
+    post_norms: bool = False        # a norm behind the attention and the MLP block too, in front of the residual sum
+    residual_scale: float = 1.0     # of a block's output where it joins the residual
+    norm_offset: float = 0.0        # added to the weights of the norms around the blocks
+
+    @property
+    def fused_norms(self) -> bool:
+        """Whether the norms and residual sums between blocks go through ``norms.residual_norms``."""
+        return self.post_norms or self.residual_scale != 1.0 or self.norm_offset != 0.0
 
     @property
     def param_count(self) -> int:
         qkv = self.hidden * (self.num_q_heads + 2 * self.num_kv_heads) * self.head_dim
         o = self.num_q_heads * self.head_dim * self.hidden
         mlp = 3 * self.hidden * self.ffn
-        return self.num_layers * (qkv + o + mlp + 2 * self.hidden + 2 * self.head_dim) + 2 * self.vocab * self.hidden + self.hidden
+        return self.num_layers * (qkv + o + mlp + (4 if self.post_norms else 2) * self.hidden + 2 * self.head_dim) + 2 * self.vocab * self.hidden + self.hidden
 
 
 class SyntheticDecoder:
@@ -64,12 +77,17 @@ class SyntheticDecoder:
         qkv_out = (s.num_q_heads + 2 * s.num_kv_heads) * s.head_dim
         self.embed = w(s.vocab, s.hidden, std=0.02)
         self.lm_head = w(s.vocab, s.hidden, std=0.02)
-        self.final_norm = torch.ones(s.hidden, device=self.device, dtype=dtype)
+        ones = lambda: torch.full((s.hidden,), 1.0 - s.norm_offset, device=self.device, dtype=dtype)      # noqa: E731
+        self.final_norm = ones()
+        self.slopes = (torch.exp2(-8.0 * torch.arange(1, s.num_q_heads + 1, dtype=torch.float32, device=self.device) / s.num_q_heads)
+                       if s.distance_bias else None)
         self.layers: List[dict] = []
         for _ in range(s.num_layers):
             self.layers.append(dict(
-                in_norm=torch.ones(s.hidden, device=self.device, dtype=dtype),
-                post_norm=torch.ones(s.hidden, device=self.device, dtype=dtype),
+                in_norm=ones(),
+                post_norm=ones(),
+                attn_out_norm=ones() if s.post_norms else None,
+                mlp_out_norm=ones() if s.post_norms else None,
                 w_qkv=w(qkv_out, s.hidden, std=s.hidden ** -0.5),
                 w_o=w(s.hidden, s.num_q_heads * s.head_dim, std=(s.num_q_heads * s.head_dim) ** -0.5 / 6),
                 w_gate_up=w(2 * s.ffn, s.hidden, std=s.hidden ** -0.5),
@@ -89,7 +107,8 @@ class SyntheticDecoder:
 
     # ---- batch state -------------------------------------------------------------------------------------
     def attach_batch(self, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
-                     ctx_lens: torch.Tensor, token_ids: torch.Tensor, active: Optional[torch.Tensor] = None) -> None:
+                     ctx_lens: torch.Tensor, token_ids: torch.Tensor, active: Optional[torch.Tensor] = None,
+                     group_offsets: Optional[torch.Tensor] = None, shared_lens: Optional[torch.Tensor] = None) -> None:
         """``k_cache``/``v_cache`` ``[L, blocks, Hkv, B, D]`` (the reference's pool layout, model_runner.py:24-31),
         ``block_tables`` int32 ``[S, max_blk]`` with room for the tokens to come, ``ctx_lens`` int32 ``[S]`` tokens
         already in the pool, ``token_ids`` int64 ``[S]`` the tokens to feed first.
@@ -98,7 +117,11 @@ class SyntheticDecoder:
         a step advances only the rows whose entry is 1.  An idle slot keeps ``seq_lens == 0`` (its attention row is
         zero) and position 0 of whatever block its table row names, so give idle rows a block nobody reads.  The
         four state tensors (``block_tables``, ``positions``, ``seq_lens``, ``active``) and ``token_ids`` may be
-        rewritten in place between steps — also between replays of a captured step."""
+        rewritten in place between steps — also between replays of a captured step.
+
+        ``group_offsets`` and ``shared_lens`` (int32 ``[groups + 1]`` and ``[groups]``) name the sequences whose tables begin
+        with the same pages: layers whose scores are not shaped then attend with
+        ``paged_kernels.paged_shared_prefix_attention``.  They may be rewritten in place too."""
         s = self.shape
         if k_cache.dim() != 5 or k_cache.size(0) != s.num_layers or k_cache.size(2) != s.num_kv_heads or k_cache.size(4) != s.head_dim:
             raise RuntimeError("k_cache must be [num_layers, blocks, Hkv, B, D] for this decoder's shape")
@@ -107,6 +130,9 @@ class SyntheticDecoder:
         self.block_tables = block_tables
         self.positions = ctx_lens.clone()                       # slot of the token being fed
         self.active = active
+        if (group_offsets is None) != (shared_lens is None):
+            raise RuntimeError("group_offsets and shared_lens belong together")
+        self.group_offsets, self.shared_lens = group_offsets, shared_lens
         self.seq_lens = ctx_lens + 1 if active is None else (ctx_lens + 1) * active
         self.token_ids = token_ids.clone()
         S = token_ids.numel()
@@ -119,9 +145,54 @@ class SyntheticDecoder:
         """Drops the batch state, the pools and the captured step (and with it the memory the capture holds)."""
         self._graph = None
         for name in ("k_cache", "v_cache", "block_tables", "positions", "seq_lens", "active", "token_ids", "q_rot",
-                     "attn_out", "uniforms", "logits"):
+                     "attn_out", "uniforms", "logits", "group_offsets", "shared_lens"):
             if hasattr(self, name):
                 delattr(self, name)
+
+    # ---- what the layers share ---------------------------------------------------------------------------------
+    def _score_shape(self, layer: int) -> dict:
+        """The shaping of a layer's scores as keyword arguments; empty when it has none."""
+        s = self.shape
+        window = s.window if s.window and layer % s.window_every == 0 else 0
+        if not (s.score_cap or s.distance_bias or window):
+            return {}
+        return dict(score_cap=s.score_cap, distance_slopes=self.slopes, window=window)
+
+    def _layers(self, x: torch.Tensor, attend, after_layer=None) -> torch.Tensor:
+        """All layers over token rows ``x``; ``attend(layer index, layer, qkv)`` returns the attention block's rows.  Returns what
+        the final norm reads — or its result, when the norms are fused with the residual sums."""
+        s = self.shape
+        fused = s.fused_norms
+        if fused:
+            first = self.layers[0]["in_norm"] if self.layers else self.final_norm
+            h = F.rms_norm(x.float(), (s.hidden,), first.float() + s.norm_offset, s.eps).to(self.dtype)
+        for li, L in enumerate(self.layers):
+            if not fused:
+                h = F.rms_norm(x, (s.hidden,), L["in_norm"], s.eps)
+            attn = attend(li, L, F.linear(h, L["w_qkv"]))
+            if after_layer is not None:
+                after_layer(li)
+            y = F.linear(attn, L["w_o"])
+            if fused:
+                x, h = norms.residual_norms(y, x, L["post_norm"], post_weight=L["attn_out_norm"], residual_scale=s.residual_scale, eps=s.eps,
+                                            weight_offset=s.norm_offset, residual_out=x, out=y)
+            else:
+                x = x + y
+                h = F.rms_norm(x, (s.hidden,), L["post_norm"], s.eps)
+            gu = F.linear(h, L["w_gate_up"])
+            y = F.linear(F.silu(gu[:, :s.ffn]) * gu[:, s.ffn:], L["w_down"])
+            if fused:
+                following = self.layers[li + 1]["in_norm"] if li + 1 < len(self.layers) else self.final_norm
+                x, h = norms.residual_norms(y, x, following, post_weight=L["mlp_out_norm"], residual_scale=s.residual_scale, eps=s.eps,
+                                            weight_offset=s.norm_offset, residual_out=x, out=y)
+            else:
+                x = x + y
+        return h if fused else x
+
+    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+        """Logits of rows that :meth:`_layers` returned."""
+        s = self.shape
+        return F.linear(x if s.fused_norms else F.rms_norm(x, (s.hidden,), self.final_norm, s.eps), self.lm_head)
 
     # ---- one decode step -----------------------------------------------------------------------------------
     def _forward(self) -> None:
@@ -132,22 +203,27 @@ class SyntheticDecoder:
         cos = self.cos_table.index_select(0, self.positions)
         sin = self.sin_table.index_select(0, self.positions)
         max_blk = self.block_tables.size(1)
-        for li, L in enumerate(self.layers):
-            h = F.rms_norm(x, (s.hidden,), L["in_norm"], s.eps)
-            qkv = F.linear(h, L["w_qkv"])
+
+        def attend(li, L, qkv):
             q = qkv[:, :hq_d].view(S, s.num_q_heads, s.head_dim)
             k = qkv[:, hq_d:hq_d + hkv_d].view(S, s.num_kv_heads, s.head_dim)
             v = qkv[:, hq_d + hkv_d:].view(S, s.num_kv_heads, s.head_dim)
-            paged_kernels.paged_qk_norm_rope_store(q, k, v, cos, sin, self.k_cache[li], self.v_cache[li],
-                                                   self.block_tables, self.positions, L["q_norm"], L["k_norm"],
+            kc, vc = self.k_cache[li], self.v_cache[li]
+            paged_kernels.paged_qk_norm_rope_store(q, k, v, cos, sin, kc, vc, self.block_tables, self.positions, L["q_norm"], L["k_norm"],
                                                    s.eps, q_out=self.q_rot)
-            paged_kernels.paged_attention_forward(self.attn_out, self.q_rot, self.k_cache[li], self.v_cache[li],
-                                                  self.block_tables, self.seq_lens, self.scale, self.block_size, max_blk)
-            x = x + F.linear(self.attn_out.view(S, hq_d), L["w_o"])
-            h = F.rms_norm(x, (s.hidden,), L["post_norm"], s.eps)
-            gu = F.linear(h, L["w_gate_up"])
-            x = x + F.linear(F.silu(gu[:, :s.ffn]) * gu[:, s.ffn:], L["w_down"])
-        logits = F.linear(F.rms_norm(x, (s.hidden,), self.final_norm, s.eps), self.lm_head)
+            shape = self._score_shape(li)
+            if shape:
+                paged_kernels.paged_scored_attention(self.attn_out, self.q_rot, kc, vc, self.block_tables, self.seq_lens, self.scale,
+                                                     self.block_size, max_blk, **shape)
+            elif self.group_offsets is not None:
+                paged_kernels.paged_shared_prefix_attention(self.attn_out, self.q_rot, kc, vc, self.block_tables, self.seq_lens,
+                                                            self.group_offsets, self.shared_lens, self.scale, self.block_size, max_blk)
+            else:
+                paged_kernels.paged_attention_forward(self.attn_out, self.q_rot, kc, vc, self.block_tables, self.seq_lens, self.scale,
+                                                      self.block_size, max_blk)
+            return self.attn_out.view(S, hq_d)
+
+        logits = self._logits(self._layers(x, attend))
         self.logits = logits
         if self.top_k > 1:
             self.uniforms.uniform_()
@@ -189,8 +265,9 @@ class SyntheticDecoder:
 
     def launches_per_step(self) -> int:
         """This library's kernels per step: one fused norm/rotary/store and one attention launch per layer, and
-        the sampler."""
-        return 2 * self.shape.num_layers + 1
+        the sampler; two launches more per layer when the norms are fused with the residual sums.  (An attention call
+        that shares prefixes is up to three launches and counted as one.)"""
+        return (4 if self.shape.fused_norms else 2) * self.shape.num_layers + 1
 
     # ---- one scheduler step with prompt chunks and decode sequences -----------------------------------------
     def mixed_step(self, ctx: dict, token_ids: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -217,21 +294,17 @@ class SyntheticDecoder:
         sin = self.sin_table.index_select(0, positions)
         hq_d, hkv_d = s.num_q_heads * s.head_dim, s.num_kv_heads * s.head_dim
         x = self.embed.index_select(0, token_ids)
-        for li, L in enumerate(self.layers):
-            h = F.rms_norm(x, (s.hidden,), L["in_norm"], s.eps)
-            qkv = F.linear(h, L["w_qkv"])
+
+        def attend(li, L, qkv):
             q = qkv[:, :hq_d].view(total, s.num_q_heads, s.head_dim)
             k = qkv[:, hq_d:hq_d + hkv_d].view(total, s.num_kv_heads, s.head_dim)
             v = qkv[:, hq_d + hkv_d:].view(total, s.num_kv_heads, s.head_dim)
             attn = paged_forward.paged_attention_step_fused(sc, q, k, v, cos, sin, k_cache[li], v_cache[li], self.scale,
-                                                            L["q_norm"], L["k_norm"], s.eps, overlap=overlap)
-            if after_layer is not None:
-                after_layer(li)
-            x = x + F.linear(attn.view(total, hq_d), L["w_o"])
-            h = F.rms_norm(x, (s.hidden,), L["post_norm"], s.eps)
-            gu = F.linear(h, L["w_gate_up"])
-            x = x + F.linear(F.silu(gu[:, :s.ffn]) * gu[:, s.ffn:], L["w_down"])
+                                                            L["q_norm"], L["k_norm"], s.eps, overlap=overlap, **self._score_shape(li))
+            return attn.view(total, hq_d)
+
+        x = self._layers(x, attend, after_layer)
         last_rows = [off + n - 1 for off, n in zip(sc.prefill_offsets, sc.prefill_tokens)]
         last_rows += list(range(sc.num_prefill_tokens, total))
         rows = torch.tensor(last_rows, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True)
-        return F.linear(F.rms_norm(x.index_select(0, rows), (s.hidden,), self.final_norm, s.eps), self.lm_head)
+        return self._logits(x.index_select(0, rows))

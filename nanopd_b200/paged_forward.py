@@ -152,8 +152,13 @@ def _sm_split(sc: StepContext, hq: int, hkv: int, d: int, elem: int, sms: int) -
     return best
 
 
-def _attend(sc: StepContext, out, q_tokens_major, k_cache, v_cache, scale, overlap: bool):
+def _attend(sc: StepContext, out, q_tokens_major, k_cache, v_cache, scale, overlap: bool, score_cap: float = 0.0,
+            distance_slopes: Optional[torch.Tensor] = None, window: int = 0):
     """Prompt-chunk attention over rows [:P] and decode attention over rows [P:] of token-major queries."""
+    shaped = score_cap != 0 or distance_slopes is not None or window != 0
+    shape = dict(score_cap=score_cap, distance_slopes=distance_slopes, window=window) if shaped else {}
+    prefill_op = paged_kernels.paged_scored_prefill_attention if shaped else paged_kernels.paged_prefill_attention
+    decode_op = paged_kernels.paged_scored_attention if shaped else paged_kernels.paged_attention_forward
     P, Dn = sc.num_prefill_tokens, sc.num_decode_tokens
     bs = k_cache.size(2)
     _, hq, d = q_tokens_major.shape
@@ -162,14 +167,12 @@ def _attend(sc: StepContext, out, q_tokens_major, k_cache, v_cache, scale, overl
     share = _sm_split(sc, hq, k_cache.size(1), d, q_tokens_major.element_size(), sms) if overlap else None
 
     def prefill(max_ctas=0):
-        paged_kernels.paged_prefill_attention(out[:P], q_tokens_major[:P], k_cache, v_cache, sc.prefill_tables,
-                                              sc.prefill_offsets, sc.prefill_tokens, sc.prefill_starts,
-                                              scale, bs, sc.prefill_tables.size(1), max_ctas=max_ctas)
+        prefill_op(out[:P], q_tokens_major[:P], k_cache, v_cache, sc.prefill_tables, sc.prefill_offsets, sc.prefill_tokens,
+                   sc.prefill_starts, scale, bs, sc.prefill_tables.size(1), max_ctas=max_ctas, **shape)
 
     def decode(max_ctas=0):
-        paged_kernels.paged_attention_forward(out[P:], q_tokens_major[P:], k_cache, v_cache, sc.decode_tables,
-                                              sc.decode_seq_lens, scale, bs, sc.decode_tables.size(1),
-                                              max_ctas=max_ctas)
+        decode_op(out[P:], q_tokens_major[P:], k_cache, v_cache, sc.decode_tables, sc.decode_seq_lens, scale, bs,
+                  sc.decode_tables.size(1), max_ctas=max_ctas, **shape)
 
     if share is None:
         if P > 0:
@@ -190,7 +193,8 @@ def _attend(sc: StepContext, out, q_tokens_major, k_cache, v_cache, scale, overl
 
 def paged_attention_step(sc: StepContext, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          k_cache: torch.Tensor, v_cache: torch.Tensor, scale: float,
-                         overlap: bool = True) -> torch.Tensor:
+                         overlap: bool = True, score_cap: float = 0.0, distance_slopes: Optional[torch.Tensor] = None,
+                         window: int = 0) -> torch.Tensor:
     """Store + attention of one layer for one step.
 
     ``q`` is ``[1, Hq, total, D]``, ``k``/``v`` ``[1, Hkv, total, D]`` after the rotary embedding (the tensors
@@ -200,7 +204,8 @@ def paged_attention_step(sc: StepContext, q: torch.Tensor, k: torch.Tensor, v: t
     (model_runner.py:210) — with one difference the reference's tests do not cover: a chunk with
     ``start_position > 0`` attends to the earlier chunks' keys in the pages as well.
     In a mixed step the two attention kernels run side by side on two streams, each on its share of the SMs
-    (``overlap=False`` runs them in turn).
+    (``overlap=False`` runs them in turn).  ``score_cap``, ``distance_slopes`` and ``window`` shape the scores of prompts and
+    decode sequences alike, as ``paged_kernels.paged_scored_attention`` describes.
     """
     P, Dn = sc.num_prefill_tokens, sc.num_decode_tokens
     total = P + Dn
@@ -215,14 +220,15 @@ def paged_attention_step(sc: StepContext, q: torch.Tensor, k: torch.Tensor, v: t
                                          sc.prefill_tables[i:i + 1].expand(n, -1), sc.prefill_positions[off:off + n])
     if Dn > 0:
         paged_kernels.paged_kv_store(k_cache, v_cache, k[0, :, P:], v[0, :, P:], sc.decode_tables, sc.decode_positions)
-    _attend(sc, out, q[0].transpose(0, 1).contiguous(), k_cache, v_cache, scale, overlap)
+    _attend(sc, out, q[0].transpose(0, 1).contiguous(), k_cache, v_cache, scale, overlap, score_cap, distance_slopes, window)
     return out.view(1, total, hq * d)
 
 
 def paged_attention_step_fused(sc: StepContext, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                scale: float, q_norm_weight=None, k_norm_weight=None, eps: float = 1e-6,
-                               overlap: bool = True) -> torch.Tensor:
+                               overlap: bool = True, score_cap: float = 0.0, distance_slopes: Optional[torch.Tensor] = None,
+                               window: int = 0) -> torch.Tensor:
     """The same step starting one stage earlier: from the projection outputs.
 
     ``q`` ``[total, Hq, D]``, ``k``/``v`` ``[total, Hkv, D]`` are the token-major views of ``q_proj``/``k_proj``/
@@ -230,7 +236,8 @@ def paged_attention_step_fused(sc: StepContext, q: torch.Tensor, k: torch.Tensor
     the rotary embedding; ``cos``/``sin`` ``[total, D]`` are the rotary tables of the step's positions.  Norm,
     rotary embedding and the store run as one launch per prompt chunk plus one for all decode tokens
     (``paged_qk_norm_rope_store``), the rotated queries stay token-major, and the attention kernels read them
-    in place: no transposes, no ``contiguous()`` copies.  Returns ``[1, total, Hq*D]``.
+    in place: no transposes, no ``contiguous()`` copies.  Returns ``[1, total, Hq*D]``.  The scores may be shaped as in
+    :func:`paged_attention_step`.
     """
     P, Dn = sc.num_prefill_tokens, sc.num_decode_tokens
     total = P + Dn
@@ -251,5 +258,5 @@ def paged_attention_step_fused(sc: StepContext, q: torch.Tensor, k: torch.Tensor
         paged_kernels.paged_qk_norm_rope_store(
             q[P:], k[P:], v[P:], cos[P:], sin[P:], k_cache, v_cache, sc.decode_tables, sc.decode_positions,
             q_norm_weight, k_norm_weight, eps, q_out=q_rot[P:])
-    _attend(sc, out, q_rot, k_cache, v_cache, scale, overlap)
+    _attend(sc, out, q_rot, k_cache, v_cache, scale, overlap, score_cap, distance_slopes, window)
     return out.view(1, total, hq * d)
