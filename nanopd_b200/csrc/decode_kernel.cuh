@@ -69,6 +69,7 @@ struct DecodeParams {
     long long bt_row_stride;
     int num_workers;
     int num_stages;
+    int block_shift, box_shift;      // log2 of block_size and box_rows (kScored and kTail)
     int seg_cost;         // see unit_at; kScored and kTail
     // kScored: scores are shaped before the softmax (all in the log2 domain)
     float cap_in;         // 2 log2(e) * scale / cap, the exponent's factor in tanh; 0 = scores are not capped
@@ -811,21 +812,58 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
     auto issue_tile = [&](int stage) {
         // Executed by the whole warp (uniform), the copies by lane 0.
         const int tok0 = (MODE == kPlain ? pc.t : pc.first + pc.t) * kTile;
+        const uint32_t bar = smem_u32(bars + stage);
+        const uint32_t kdst = smem_u32(stage_base + (size_t)stage * STAGE_BYTES);
+        const uint32_t vdst = kdst + TILE_BYTES;
+        if constexpr (MODE != kPlain) {
+            // A warp issues an instruction every seven clocks or so here (fixed latencies, little to overlap), so the tile's
+            // time is its instruction count: block sizes are powers of two (no divisions), and the boxes go out one per lane
+            // in one instruction of the warp.
+            constexpr int kPerBox = 2 * NH;                      // K and V, 64-element slabs
+            const int my_k = lane / kPerBox, my_hf = lane % kPerBox / 2;
+            const int npages = (pc.len + p.block_size - 1) >> p.block_shift;
+            const int phys_head = p.kv_rep == 1 ? pc.h : pc.h / p.kv_rep;
+            int my_id = 0, first_box = 0, boxes = 1;
+            auto checked = [&](int id) {
+                if (id < 0 || id >= p.num_blocks) {
+                    if (lane == 0) atomicOr(p.status, NPD_STATUS_BAD_BLOCK_ID);
+                    id = p.num_blocks;   // out of bounds for the tensor map: the box is zero-filled
+                }
+                return id;
+            };
+            if (p.box_rows == kTile) {
+                my_id = checked(table_lookup(win, pc.s, tok0 >> p.block_shift, npages, lane, p));
+            } else {
+                // several boxes to a tile; those wholly before the window or behind the sequence are not read
+                boxes = min(kTile, pc.len - tok0 + p.box_rows - 1) >> p.box_shift;
+                if (MODE == kScored) first_box = max(0, first_visible<MODE>(p, pc.len) - tok0) >> p.box_shift;
+                for (int k = first_box; k < boxes; ++k) {
+                    const int id = checked(table_lookup(win, pc.s, (tok0 + (k << p.box_shift)) >> p.block_shift, npages, lane, p));
+                    if (k == my_k) my_id = id;
+                }
+            }
+            const int my_row = phys_head * p.block_size + ((tok0 + my_k * p.box_rows) & (p.block_size - 1));
+            fence_proxy_async_smem();
+            if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>((boxes - first_box) * 2 * NH * p.box_rows * 128));
+            __syncwarp();
+            if (my_k >= first_box && my_k < boxes)
+                tma_load_3d((lane & 1 ? vdst : kdst) + static_cast<uint32_t>((my_k * NH + my_hf) * half_bytes),
+                            lane & 1 ? &tm_v : &tm_k, bar, my_hf * 64, my_row, my_id);
+            __syncwarp();
+            ++issued;
+            if (issued < my_tiles) cursor_advance<MODE>(pc, pre, p);
+            return;
+        }
         const int npages = (pc.len + p.block_size - 1) / p.block_size;
         const int nbox_total = kTile / p.box_rows;
         int nbox = 0;
         for (int k = 0; k < nbox_total; ++k) nbox += (tok0 + k * p.box_rows < pc.len) ? 1 : 0;
-        // boxes wholly before the window are not read: their pages may have been given away
-        const int box0 = MODE == kScored ? max(0, first_visible<MODE>(p, pc.len) - tok0) / p.box_rows : 0;
-        const uint32_t bar = smem_u32(bars + stage);
-        const uint32_t kdst = smem_u32(stage_base + (size_t)stage * STAGE_BYTES);
-        const uint32_t vdst = kdst + TILE_BYTES;
         const int phys_head = pc.h / p.kv_rep;
         if (lane == 0) {
             fence_proxy_async_smem();
-            mbar_expect_tx(bar, static_cast<uint32_t>((nbox - box0) * 2 * NH * p.box_rows * 128));
+            mbar_expect_tx(bar, static_cast<uint32_t>(nbox * 2 * NH * p.box_rows * 128));
         }
-        for (int k = box0; k < nbox; ++k) {
+        for (int k = 0; k < nbox; ++k) {
             const int token = tok0 + k * p.box_rows;
             const int page = token / p.block_size;
             const int row_in_page = token - page * p.block_size;
@@ -1496,6 +1534,9 @@ int run_decode(const DecodeCall &c) {
     p.cap_log2 = c.score_cap * 1.4426950408889634f;
     p.slopes = c.slopes;
     p.window = c.window > 0 && c.window < INT32_MAX ? static_cast<int>(c.window) : INT32_MAX;
+    p.block_shift = p.box_shift = 2;
+    while (1 << p.block_shift < p.block_size) ++p.block_shift;
+    while (1 << p.box_shift < p.box_rows) ++p.box_shift;
     p.seg_cost = MODE == kTail ? 6 : 2;
     p.cluster = ls.cluster;
     p.group_offsets = c.group_offsets;
