@@ -11,7 +11,11 @@ extern "C" int npd_paged_prefill_attention(void *out, const void *q, const void 
                                            int64_t num_blocks, int64_t cache_block_stride, int64_t bt_row_stride,
                                            int dtype, void *workspace, size_t workspace_bytes, int flags,
                                            void *stream) {
-    return run_prefill<kCausal>({out, q, k_cache, v_cache, block_tables, chunk_q_offset_host, chunk_tokens_host, chunk_start_host,
-                                 num_chunks, scale, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
-                                 num_blocks, cache_block_stride, bt_row_stride, dtype, workspace, workspace_bytes, flags, stream});
+    try {
+        return run_prefill<kCausal>({out, q, k_cache, v_cache, block_tables, chunk_q_offset_host, chunk_tokens_host, chunk_start_host,
+                                     num_chunks, scale, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                                     num_blocks, cache_block_stride, bt_row_stride, dtype, workspace, workspace_bytes, flags, stream});
+    } catch (const std::exception &e) {          // the list of work items is host memory
+        return npd::fail(NPD_ERR_CUDA, "prefill attention: %s", e.what());
+    }
 }

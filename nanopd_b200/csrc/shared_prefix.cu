@@ -206,12 +206,12 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
     NPD_REQUIRE((flags & ~0xffff00) == 0, NPD_ERR_INVALID_ARG, "shared-prefix attention: only NPD_FLAG_MAX_CTAS is a flag here");
     const int rs = npd::check_score_shape("shared-prefix attention", scale, 0.f, nullptr, 0);
     if (rs != NPD_OK) return rs;
+    NPD_REQUIRE(num_groups >= 1 && num_groups <= kMaxGroups, NPD_ERR_INVALID_ARG, "shared-prefix attention: between 1 and %d groups", kMaxGroups);
     DecodeCall c{out, q, k_cache, v_cache, block_tables, seq_lens, scale, num_seqs, num_q_heads, num_kv_heads, head_dim,
                  block_size, max_blocks_per_seq, num_blocks, cache_block_stride, bt_row_stride, dtype, workspace,
                  workspace_bytes, flags, stream};
     int rc = check_decode_call(c);
     if (rc != NPD_OK) return rc;
-    NPD_REQUIRE(num_groups >= 1 && num_groups <= kMaxGroups, NPD_ERR_INVALID_ARG, "shared-prefix attention: between 1 and %d groups", kMaxGroups);
     if (num_seqs == 0) return NPD_OK;
     NPD_REQUIRE(group_offsets && shared_lens, NPD_ERR_INVALID_ARG, "shared-prefix attention: NULL pointer");
     const int64_t group = num_q_heads / num_kv_heads;

@@ -75,6 +75,7 @@ def release_workspaces(device=None) -> None:
             del _workspaces[k]
         for k in scratch_keys:
             del _scratch[k]
+            _scratch_at.pop(k, None)
         for k in [k for k in _captured_scratch if idx is None or k[0] == idx]:
             del _captured_scratch[k]           # the graph's own pool keeps the memory
 
@@ -175,6 +176,7 @@ def _ws_ptr(dev_index: int, handle: int, nbytes: int):
 # status bits of all of them go to one word per device, which lives as long as the process.
 # ---------------------------------------------------------------------------
 _scratch: Dict[Tuple[int, int], torch.Tensor] = {}
+_scratch_at: Dict[Tuple[int, int], Tuple[int, int]] = {}            # address and size of each, for the common path
 _packed_call = _C.npd_call_packed
 _pack_scored = struct.Struct("<q6Q2dQ11qQqQqQ").pack           # device, then the entry point's arguments
 _pack_scored_prefill = struct.Struct("<q8Qq2dQ10qQqQqQ").pack
@@ -193,6 +195,7 @@ def _packed_op(op: int, pack, *args) -> None:
 
 
 _capturing = torch._C._cuda_isCurrentStreamCapturing
+_current_device = torch._C._cuda_getDevice
 _captured_scratch: Dict[Tuple[int, int], Tuple[int, torch.Tensor, int]] = {}     # the stream's latest capture; bytes cleared
 _status_words: Dict[int, torch.Tensor] = {}
 _status_addresses: Dict[int, int] = {}
@@ -213,28 +216,34 @@ def _status_ptr(dev_index: int) -> int:
     return address
 
 
-def _scratch_for(dev_index: int, handle: int, nbytes: int, cleared: int) -> torch.Tensor:
-    """At least ``nbytes`` of scratch for a call on the current stream (``handle``), the first ``cleared`` bytes zero when
-    it is first used."""
+def _scratch_for(dev_index: int, handle: int, nbytes: int, cleared: int) -> Tuple[int, int]:
+    """Address and size of at least ``nbytes`` of scratch for a call on the stream ``handle`` of device ``dev_index``, the first
+    ``cleared`` bytes zero when it is first used."""
     key = (dev_index, handle)
-    if _capturing():
-        capture = ctypes.c_uint64(0)
-        _lib.check(_C.npd_capture_id(handle, ctypes.byref(capture)))
-        held = _captured_scratch.get(key)
-        if held is None or held[0] != capture.value or held[1].numel() < nbytes:
-            ws, before = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev_index)), 0
-        else:
-            ws, before = held[1], held[2]
-        if before < cleared:
-            ws[before:cleared].zero_()
-            with _ws_lock:
-                _captured_scratch[key] = (capture.value, ws, cleared)
-        return ws
-    ws = _scratch.get(key)
-    if ws is None or ws.numel() < nbytes:
+    capture_id = 0
+    if _capturing() or _current_device() != dev_index:          # the first asks about the current device's stream only
+        found = ctypes.c_uint64(0)
+        _lib.check(_C.npd_capture_id(handle, ctypes.byref(found)))
+        capture_id = found.value
+    if capture_id == 0:
+        at = _scratch_at.get(key)
+        if at is not None and at[1] >= nbytes:
+            return at
         with _ws_lock:
-            _scratch[key] = ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev_index))
-    return ws
+            ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev_index))
+            _scratch[key] = ws
+            _scratch_at[key] = at = (ws.data_ptr(), ws.numel())
+        return at
+    held = _captured_scratch.get(key)
+    if held is None or held[0] != capture_id or held[1].numel() < nbytes:
+        ws, before = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev_index)), 0
+    else:
+        ws, before = held[1], held[2]
+    if before < cleared:
+        ws[before:cleared].zero_()
+        with _ws_lock:
+            _captured_scratch[key] = (capture_id, ws, cleared)
+    return ws.data_ptr(), ws.numel()
 
 
 def _cache_geometry(cache: torch.Tensor, name: str):
@@ -627,17 +636,18 @@ def paged_scored_attention(out, query, key_cache, value_cache, block_tables, seq
         _remember(_scored_plans, key, plan)
     dev_index, need, cleared, flags, cap, win, args = plan
     handle = _raw_stream(dev_index)
-    ws = _scratch_for(dev_index, handle, need, cleared)
+    ws, ws_bytes = _scratch_for(dev_index, handle, need, cleared)
     _packed_op(_lib.NPD_OP_SCORED_ATTENTION, _pack_scored,
         dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-        scale, cap, 0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws.data_ptr(), ws.numel(),
-        _status_ptr(dev_index), flags, handle)
+        scale, cap, 0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws, ws_bytes,
+        _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
 # (2d) decode attention for a batch that shares prefixes
 # ---------------------------------------------------------------------------
 _shared_plans: Dict[tuple, tuple] = {}
+_scored_prefill_plans: Dict[tuple, tuple] = {}
 
 
 def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tables, seq_lens, group_offsets, shared_lens,
@@ -682,10 +692,10 @@ def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tabl
         _remember(_shared_plans, key, plan)
     dev_index, need, cleared, flags, args = plan
     handle = _raw_stream(dev_index)
-    ws = _scratch_for(dev_index, handle, need, cleared)
+    ws, ws_bytes = _scratch_for(dev_index, handle, need, cleared)
     _packed_op(_lib.NPD_OP_SHARED_PREFIX_ATTENTION, _pack_shared,
         dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-        group_offsets.data_ptr(), shared_lens.data_ptr(), scale, *args, ws.data_ptr(), ws.numel(), _status_ptr(dev_index), flags, handle)
+        group_offsets.data_ptr(), shared_lens.data_ptr(), scale, *args, ws, ws_bytes, _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
@@ -703,41 +713,54 @@ def paged_scored_prefill_attention(out, query, key_cache, value_cache, block_tab
     """
     name = "paged_scored_prefill_attention"
     try:
-        _require(query.is_cuda and query.dim() == 3, f"{name}: query must be a CUDA tensor [tokens, num_heads, head_size]")
-        _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2, f"{name}: block_tables must be int32 [chunks, max_blk]")
-        dev = query.device
-        total, hq, d = query.shape
-        nchunks = len(chunk_tokens)
         offs, toks, starts = array("i", chunk_q_offsets), array("i", chunk_tokens), array("i", chunk_starts)
-        _require(len(offs) == nchunks and len(starts) == nchunks and block_tables.size(0) == nchunks,
-                 f"{name}: one offset, token count, start position and table row per chunk")
-        _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and query.is_contiguous() and out.is_contiguous(),
-                 f"{name}: out must match query in shape, dtype and device; both contiguous")
-        _require(query.dtype in (torch.float16, torch.bfloat16), f"{name}: unsupported dtype {query.dtype}")
-        nb, hkv, bs, cd, cstride = _cache_geometry(key_cache, "key_cache")
-        _require(_cache_geometry(value_cache, "value_cache") == (nb, hkv, bs, cd, cstride), "cache layouts differ")
-        _require(cd == d and int(block_size) == bs and key_cache.dtype == query.dtype == value_cache.dtype, f"{name}: cache does not match query")
-        _require(all(t.device == dev for t in (key_cache, value_cache, block_tables)), f"{name}: all tensors must be on the query's device")
-        _require(hq % hkv == 0, "num_heads must be a multiple of num_kv_heads")
-        _require(block_tables.stride(1) == 1 or block_tables.size(1) == 1, "block_tables rows must be contiguous")
-        max_blk = int(max_num_blocks_per_seq)
-        _require(1 <= max_blk <= block_tables.size(1), "max_num_blocks_per_seq out of range")
-        _require(0 <= int(max_ctas) <= 0xffff, "max_ctas out of range")
-        _score_shape(name, score_cap, distance_slopes, window, hq, dev)
+        key = (out.shape, out.stride(), out.dtype, out.device, query.shape, query.stride(), query.dtype, query.device,
+               key_cache.shape, key_cache.stride(), key_cache.dtype, key_cache.device, value_cache.shape, value_cache.stride(),
+               value_cache.dtype, value_cache.device, block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.device,
+               block_size, max_num_blocks_per_seq, None if distance_slopes is None else _sig(distance_slopes), score_cap, window, max_ctas)
+        plan = _scored_prefill_plans.get(key)
+        if plan is None:
+            _require(query.is_cuda and query.dim() == 3, f"{name}: query must be a CUDA tensor [tokens, num_heads, head_size]")
+            _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2, f"{name}: block_tables must be int32 [chunks, max_blk]")
+            dev = query.device
+            _, hq, d = query.shape
+            _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and query.is_contiguous() and out.is_contiguous(),
+                     f"{name}: out must match query in shape, dtype and device; both contiguous")
+            _require(query.dtype in (torch.float16, torch.bfloat16), f"{name}: unsupported dtype {query.dtype}")
+            nb, hkv, bs, cd, cstride = _cache_geometry(key_cache, "key_cache")
+            _require(_cache_geometry(value_cache, "value_cache") == (nb, hkv, bs, cd, cstride), "cache layouts differ")
+            _require(cd == d and int(block_size) == bs and key_cache.dtype == query.dtype == value_cache.dtype, f"{name}: cache does not match query")
+            _require(all(t.device == dev for t in (key_cache, value_cache, block_tables)), f"{name}: all tensors must be on the query's device")
+            _require(hq % hkv == 0, "num_heads must be a multiple of num_kv_heads")
+            _require(block_tables.stride(1) == 1 or block_tables.size(1) == 1, "block_tables rows must be contiguous")
+            max_blk = int(max_num_blocks_per_seq)
+            _require(1 <= max_blk <= block_tables.size(1), "max_num_blocks_per_seq out of range")
+            _require(0 <= int(max_ctas) <= 0xffff, "max_ctas out of range")
+            _score_shape(name, score_cap, distance_slopes, window, hq, dev)
+            row_stride = block_tables.stride(0) if block_tables.size(0) > 1 else block_tables.size(1)
+            plan = (dev.index, query.size(0), max_blk * bs, block_tables.size(0), float(score_cap), int(window),
+                    (hq, hkv, d, bs, max_blk, nb, cstride, row_stride, _DTYPE_CODE[query.dtype]), int(max_ctas) << 8)
+            _remember(_scored_prefill_plans, key, plan)
     except (AttributeError, TypeError, OverflowError):
         raise RuntimeError(f"{name} takes tensors, lists of whole numbers and numbers") from None
+    dev_index, total, capacity, rows, cap, win, args, flags = plan
+    nchunks = len(toks)
+    _require(len(offs) == nchunks and len(starts) == nchunks and rows == nchunks,
+             f"{name}: one offset, token count, start position and table row per chunk")
     for off, n, start in zip(offs, toks, starts):
-        _require(n >= 0 and off >= 0 and off + n <= total and start >= 0, f"{name}: chunk outside the query tensor")
-        _require(start + n <= max_blk * bs, f"{name}: chunk reaches beyond its block table")
+        if n < 0 or off < 0 or off + n > total or start < 0:
+            raise RuntimeError(f"{name}: chunk outside the query tensor")
+        if start + n > capacity:
+            raise RuntimeError(f"{name}: chunk reaches beyond its block table")
     if nchunks == 0 or total == 0:
         return
-    handle = _raw_stream(dev.index)
-    ws = _scratch_for(dev.index, handle, 256, 256)
+    handle = _raw_stream(dev_index)
+    ws, ws_bytes = _scratch_for(dev_index, handle, 256, 256)
     _packed_op(_lib.NPD_OP_SCORED_PREFILL_ATTENTION, _pack_scored_prefill,
-        dev.index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-        offs.buffer_info()[0], toks.buffer_info()[0], starts.buffer_info()[0], nchunks, scale, score_cap,
-        0 if distance_slopes is None else distance_slopes.data_ptr(), int(window), hq, hkv, d, bs, max_blk, nb, cstride, block_tables.stride(0),
-        _DTYPE_CODE[query.dtype], ws.data_ptr(), ws.numel(), _status_ptr(dev.index), int(max_ctas) << 8, handle)
+        dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+        offs.buffer_info()[0], toks.buffer_info()[0], starts.buffer_info()[0], nchunks, scale, cap,
+        0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws, ws_bytes,
+        _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------

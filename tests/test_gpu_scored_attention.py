@@ -259,3 +259,34 @@ def test_scales_that_are_refused(kernels, scale):
 def test_a_scale_of_zero_weighs_every_key_alike(kernels):
     q, kc, vc, bt, sl, _ = make([20, 300], 12, 2, 128, 16, torch.float16)
     check(kernels, q, kc, vc, bt, sl, 0.0, 5.0, None, 100)
+
+
+def test_more_sequences_than_a_launch_takes(kernels):
+    lens = [1 + i % 70 for i in range(5000)]
+    q, kc, vc, bt, sl, scale = make(lens, 4, 2, 64, 16, torch.float16)
+    check(kernels, q, kc, vc, bt, sl, scale, 6.0, slopes_for(4), 33)
+
+
+def test_a_larger_call_after_a_smaller_one_in_one_capture(kernels):
+    """The capture's scratch grows with its calls: more sequences need more cleared tickets."""
+    small = make([3000, 2500], 32, 8, 128, 16, torch.bfloat16)
+    large = make([700 + 13 * i for i in range(64)], 32, 8, 128, 16, torch.bfloat16, seed=1)
+    want = [check(kernels, *st, 50.0, max_ctas=140) for st in (small, large)]
+    outs = [torch.empty_like(w) for w in want]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for st, o in zip((small, large, small), outs + [outs[0]]):
+            q, kc, vc, bt, sl, scale = st
+            kernels.paged_scored_attention(o, q, kc, vc, bt, sl, scale, 16, bt.size(1), score_cap=50.0, max_ctas=140)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_workspaces_are_dropped_and_made_again(kernels):
+    q, kc, vc, bt, sl, scale = make([3000, 17], 32, 8, 128, 16, torch.bfloat16)
+    want = check(kernels, q, kc, vc, bt, sl, scale, 50.0, max_ctas=140)
+    from nanopd_b200 import paged_kernels
+    paged_kernels.release_workspaces(DEV)
+    assert torch.equal(check(kernels, q, kc, vc, bt, sl, scale, 50.0, max_ctas=140), want)
