@@ -31,11 +31,11 @@ struct PlanParams {
     int workers;
 };
 
-// Exclusive prefix over v[0..n) in place, v[n] = the total; the whole CTA of kPlanThreads threads.
+// Exclusive prefix over v[0..n) in place, v[n] = the total; the whole CTA.  Ends with a barrier.
 __device__ void exclusive_prefix(int *v, int n) {
-    __shared__ int warp_sums[kPlanThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int chunk = (n + kPlanThreads - 1) / kPlanThreads;
+    __shared__ int warp_sums[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+    const int chunk = (n + threads - 1) / threads;
     const int lo = min(tid * chunk, n), hi = min(lo + chunk, n);
     int sum = 0;
     for (int i = lo; i < hi; ++i) sum += v[i];
@@ -45,19 +45,12 @@ __device__ void exclusive_prefix(int *v, int n) {
         const int u = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += u;
     }
-    if (lane == 31) warp_sums[warp] = incl;
-    __syncthreads();
-    if (warp == 0) {
-        int w = warp_sums[lane], inc = w;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, d);
-            if (lane >= d) inc += u;
-        }
-        warp_sums[lane] = inc - w;
+    int run = incl - sum;
+    if (n > 32 * chunk) {                        // more than the first warp has some
+        if (lane == 31) warp_sums[warp] = incl;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) run += warp_sums[w];
     }
-    __syncthreads();
-    int run = warp_sums[warp] + incl - sum;
     for (int i = lo; i < hi; ++i) {
         const int x = v[i];
         v[i] = run;
@@ -72,19 +65,19 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     int *offs = plan_smem;                       // [num_groups + 1] group_offsets
     int *unit = offs + p.num_groups + 1;         // [num_groups + 1] units in front of each group
     int *least = unit + p.num_groups + 1;        // [num_groups] shortest sequence that is not empty
-    __shared__ int bad, units_per_worker;
+    __shared__ int bad;
     const int tid = threadIdx.x;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int my_len = tid < p.num_seqs ? p.seq_lens[tid] : 0;      // under way together with the offsets
     if (tid == 0) bad = 0;
-    for (int g = tid; g <= p.num_groups; g += kPlanThreads) {
+    for (int g = tid; g <= p.num_groups; g += blockDim.x) {
         offs[g] = p.group_offsets[g];
         if (g < p.num_groups) least[g] = INT32_MAX;
     }
-    __syncthreads();
+    __syncthreads();                             // `bad` and the offsets are set
     // Groups must be consecutive ranges of the batch.  Anything else shares nothing (every row is still right: the tail
     // then covers whole sequences) and is flagged.
-    for (int g = tid; g < p.num_groups; g += kPlanThreads)
+    for (int g = tid; g < p.num_groups; g += blockDim.x)
         if (offs[g] < 0 || offs[g + 1] < offs[g] || offs[g + 1] > p.num_seqs) bad = 1;
     __syncthreads();
     const bool none = bad != 0;
@@ -99,13 +92,13 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
         }
         return lo;
     };
-    for (int s = tid; s < p.num_seqs; s += kPlanThreads) {
+    for (int s = tid; s < p.num_seqs; s += blockDim.x) {
         const int n = s == tid ? my_len : p.seq_lens[s];
         const int g = group_of(s);
         if (g >= 0 && n > 0) atomicMin(least + g, n);
     }
     __syncthreads();
-    for (int g = tid; g < p.num_groups; g += kPlanThreads) {
+    for (int g = tid; g < p.num_groups; g += blockDim.x) {
         PrefixGroup out{0, 0, 0, 0};
         if (!none) {
             out.begin = offs[g];
@@ -124,13 +117,9 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     }
     __syncthreads();
     exclusive_prefix(unit, p.num_groups);
-    if (tid == 0) {
-        const int total = unit[p.num_groups];
-        units_per_worker = max(1, (total + p.workers - 1) / p.workers);
-        *p.head = PrefixPlanHead{total, units_per_worker, {0, 0}};
-    }
-    __syncthreads();
-    for (int s = tid; s < p.num_seqs; s += kPlanThreads) {
+    const int total = unit[p.num_groups], units_per_worker = max(1, (total + p.workers - 1) / p.workers);
+    if (tid == 0) *p.head = PrefixPlanHead{total, units_per_worker, {0, 0}};
+    for (int s = tid; s < p.num_seqs; s += blockDim.x) {
         PrefixSeqPlan sp{0, 0, 0, 0, 0, {0, 0, 0}};
         const int lo = group_of(s);
         if (lo >= 0) {
@@ -144,8 +133,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
         }
         p.seqs[s] = sp;
     }
-    const int total = unit[p.num_groups];
-    for (int w = tid; w < p.workers; w += kPlanThreads) {
+    for (int w = tid; w < p.workers; w += blockDim.x) {
         PrefixSeed seed{0, 0, 0, 0};
         const long long u = (long long)w * units_per_worker;
         if (u < total) {
@@ -263,7 +251,9 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
         NPD_CUDA_TRY(cudaFuncSetAttribute(shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_most));
         npd::set_up_on_device(plan_done, dev);
     }
-    shared_prefix_plan_kernel<<<1, kPlanThreads, (size_t)(3 * num_groups + 2) * sizeof(int), st>>>(pp);
+    // a barrier of 1024 threads costs more than what a batch of a few hundred sequences gives them to do
+    const int plan_threads = num_seqs <= 512 && num_groups <= 512 ? 256 : kPlanThreads;
+    shared_prefix_plan_kernel<<<1, plan_threads, (size_t)(3 * num_groups + 2) * sizeof(int), st>>>(pp);
     NPD_CUDA_TRY(cudaGetLastError());
     npd::PrefixPass pass{q, k_cache, v_cache, block_tables, scale, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
                          max_blocks_per_seq, num_blocks, cache_block_stride, bt_row_stride, dtype, status, pp.groups, pp.seeds,
