@@ -973,39 +973,18 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             const int first_pos = it.start + (x == 0 ? it.tok0[0] : it.tok0[1]);       // of the tile's first row
             // last visible key of this row
             const int pos = MODE == kPrefix ? it.ctx_end - 1 : first_pos + tq_idx;
+            // rows behind the last (token, head) of a tile hold whatever shared memory held: what their scores are must not choose
+            // the way of the warp's other rows
+            const bool row_used = row < p.tq * p.group;
             float slope2 = 0.f;                                  // kShaped: slope of this row's head, log2 domain
             if constexpr (shapes(MODE))
                 if (p.slopes != nullptr && row < p.tq * p.group) slope2 = __ldg(p.slopes + it.h * p.group + hg) * 1.4426950408889634f;
             float m_run = -INFINITY, l_run = 0.f;
-            // Before a wait for a V tile at an item's first half-step: this group may be ahead of V tiles of the item before
-            // (it never waits for them otherwise), and a parity wait for a ring stage is only sound once the stage's tile
-            // before has landed.  That one is the group's last tile of the item before when the other query tile had one
-            // tile more (it has at most one), else an older one: the group's last PV product tells.
-            auto v_phase_known = [&]() {
-                return c == 0 || wait_or_abort(smem_u32(&ctrl->pv_done[x][(c - 1) & 1]), ((c - 1) >> 1) & 1, abort_flag, p.status);
-            };
 #pragma unroll 1
             for (int u = 0; ok && u < U; ++u) {
                 const int cu = c + u, buf = cu & 1;
                 const int t = u / kHPT, gt = g + t, stage = gt % kStagesV;
                 const int key0 = t0 * kTK + u * kHalfKeys;
-                // V rows at or past ctx_end were never written (or never loaded): clear them so that P = 0
-                // there cannot meet a NaN.  Both softmax groups do it (idempotent), at the first half-step of the
-                // key tile, before they release its probabilities.
-                if (u % kHPT == 0 && (t0 + t) * kTK + kTK > it.ctx_end) {
-                    if (u == 0 && !(ok = v_phase_known())) break;
-                    if (!(ok = wait_or_abort(smem_u32(&ctrl->v_full[stage]), (gt / kStagesV) & 1, abort_flag, p.status))) break;
-                    uint8_t *v_tile = v_ring + (size_t)stage * kKvTileBytes;
-                    const int first = max(it.ctx_end - (t0 + t) * kTK, 0);
-                    constexpr int kPieces = kHalves * 8;           // 16-byte pieces per row
-                    const int n16 = (kTK - first) * kPieces;
-                    for (int idx = threadIdx.x & 127; idx < n16; idx += 128) {
-                        const int r = first + idx / kPieces, piece = idx % kPieces;
-                        *reinterpret_cast<uint4 *>(v_tile + (piece >> 3) * kKvHalfBytes + r * 128 + ((piece & 7) << 4)) =
-                            make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                }
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 20, u);
                 if (!(ok = wait_or_abort(smem_u32(&ctrl->s_full[x][buf]), (cu >> 1) & 1, abort_flag, p.status))) break;
                 if (lane == 0) NPD_TRACE(sm_role, 21, u);
@@ -1028,7 +1007,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                         m_run = m_new;                              // kCausal: key 0 is visible to every row, so it is finite
                         return true;
                     }
-                    const bool grow = m_new > m_run + kRescaleThreshold;
+                    const bool grow = m_new > m_run + kRescaleThreshold && (MODE == kCausal || row_used);
                     if (__any_sync(0xffffffffu, grow)) {
                         if (!wait_or_abort(smem_u32(&ctrl->pv_done[x][(cu - 1) & 1]), ((cu - 1) >> 1) & 1, abort_flag, p.status)) return false;
                         tc_fence_after();
@@ -1102,7 +1081,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                         if (direct) {
                             // tanh grows with its argument: the largest capped score is that of the largest raw one
                             mx = row_max(sc);
-                            direct = !__any_sync(0xffffffffu, fmaxf(mx, -row_min(sc)) >= p.cap_reach);
+                            direct = !__any_sync(0xffffffffu, row_used && fmaxf(mx, -row_min(sc)) >= p.cap_reach);
                         }
                         if (direct) {
                             if (!(ok = new_maximum(mx * cap_factor2(make_float2(mx * mx, 0.f), p).x))) break;
@@ -1136,18 +1115,31 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                     probabilities([&](float2 y) { return __ffma2_rn(y, scale2, negm2); });
                 }
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 24, u);
-                if constexpr (shapes(MODE)) {
-                    if (u == 0 && it.lo > key0) {                // V rows before the item's window may hold anything: clear them before PV reads them
-                        if (!(ok = v_phase_known())) break;
+                // V rows that no row of the item may see — at or past ctx_end, never written or never loaded; before the item's
+                // window, not loaded or no longer its own — may hold anything: clear them, so that P = 0 there cannot meet a
+                // NaN.  Both softmax groups do it (idempotent), at the first half-step of the key tile, before they release
+                // its probabilities.  Only here, behind the wait for the half-step's scores: a parity wait for a ring stage is
+                // sound once the stage's tile before has landed, and these groups wait for V tiles nowhere else.  The MMA warp
+                // that issued the scores had waited for that tile — for every tile of the items before, also of those this
+                // query tile had no part in, and for the tiles of the PV products it had issued, this half-step's last but two
+                // among them.
+                if (u % kHPT == 0) {
+                    const int tile_key0 = key0, behind_from = max(0, it.ctx_end - tile_key0);
+                    int before_to = 0;
+                    if constexpr (shapes(MODE)) before_to = u == 0 ? max(0, it.lo - tile_key0) : 0;
+                    if (behind_from < kTK || before_to > 0) {
                         if (!(ok = wait_or_abort(smem_u32(&ctrl->v_full[stage]), (gt / kStagesV) & 1, abort_flag, p.status))) break;
                         uint8_t *v_tile = v_ring + (size_t)stage * kKvTileBytes;
-                        constexpr int kPieces = kHalves * 8;
-                        const int n16 = (it.lo - key0) * kPieces;
-                        for (int idx = threadIdx.x & 127; idx < n16; idx += 128) {
-                            const int r = idx / kPieces, piece = idx % kPieces;
-                            *reinterpret_cast<uint4 *>(v_tile + (piece >> 3) * kKvHalfBytes + r * 128 + ((piece & 7) << 4)) =
-                                make_uint4(0, 0, 0, 0);
-                        }
+                        constexpr int kPieces = kHalves * 8;           // 16-byte pieces per row
+                        auto clear = [&](int first, int last) {
+                            for (int idx = threadIdx.x & 127; idx < (last - first) * kPieces; idx += 128) {
+                                const int r = first + idx / kPieces, piece = idx % kPieces;
+                                *reinterpret_cast<uint4 *>(v_tile + (piece >> 3) * kKvHalfBytes + r * 128 + ((piece & 7) << 4)) =
+                                    make_uint4(0, 0, 0, 0);
+                            }
+                        };
+                        if (before_to > 0) clear(0, before_to);
+                        if (behind_from < kTK) clear(behind_from, kTK);
                         fence_proxy_async_smem();
                     }
                 }

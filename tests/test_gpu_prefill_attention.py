@@ -6,7 +6,7 @@ import torch
 
 from conftest import TOL
 from nanopd_b200 import workloads
-from oracle import paged_oracle
+from oracle import paged_oracle, shaped_oracle
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -322,3 +322,38 @@ def test_short_items_behind_pairs_of_unequal_reach(kernels, repeat):
     kernels.paged_prefill_attention(alone, q, *args)
     torch.cuda.synchronize()
     assert torch.isfinite(out).all() and torch.equal(out, alone)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 256), (32, 8, 128), (8, 8, 64), (32, 1, 256)])
+@pytest.mark.parametrize("max_ctas", [1, 3])
+def test_partial_last_tiles_one_item_after_another(kernels, hq, hkv, d, max_ctas):
+    """Few CTAs work through many items whose last key tile is partly unwritten (NaN), items in which one query tile has no
+    part, and single-tile items between longer ones: what clears unwritten V rows must clear them in the awaited tile alone."""
+    block = 16
+    chunks = [(start, n) for start, n in ((0, 33), (500, 1), (63, 70), (0, 1), (127, 2), (200, 150), (0, 300), (65, 63), (128, 129), (1000, 20))] * 3
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(3)
+    need = [-(-(s + n) // block) for s, n in chunks]
+    kc, vc = (torch.full((sum(need), hkv, block, d), float("nan"), dtype=torch.float16, device=DEV) for _ in range(2))
+    bt = torch.zeros(len(chunks), max(need), dtype=torch.int32, device=DEV)
+    at, offs = 0, []
+    for i, (s, n) in enumerate(chunks):
+        bt[i, :need[i]] = torch.arange(at, at + need[i], device=DEV)
+        for c in (kc, vc):
+            rows = torch.randn(need[i] * block, hkv, d, generator=gen, device=DEV).to(c.dtype)
+            rows[s + n:] = float("nan")
+            c[at:at + need[i]] = rows.view(need[i], block, hkv, d).transpose(1, 2)
+        at += need[i]
+        offs.append(sum(m for _, m in chunks[:i]))
+    q = torch.randn(sum(n for _, n in chunks), hq, d, generator=gen, device=DEV).to(torch.float16)
+    args = (kc, vc, bt, offs, [n for _, n in chunks], [s for s, _ in chunks], d ** -0.5, block, bt.size(1))
+    want = torch.empty_like(q)
+    kernels.paged_prefill_attention(want, q, *args)
+    for _ in range(5):
+        out = torch.empty_like(q)
+        kernels.paged_prefill_attention(out, q, *args, max_ctas=max_ctas)
+        assert torch.isfinite(out).all() and torch.equal(out, want)
+    for i, (s, n) in enumerate(chunks[:10]):
+        exact, A, l = shaped_oracle.attend(q[offs[i]:offs[i] + n], kc, vc, bt[i], s, d ** -0.5)
+        tol = shaped_oracle.attention_tolerance(exact, A, l, s + n, q.dtype, 6.0)
+        assert ((want[offs[i]:offs[i] + n].double() - exact).abs() <= tol).all(), f"chunk {i}"

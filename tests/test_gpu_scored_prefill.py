@@ -219,3 +219,19 @@ def test_caps_far_from_the_usual(kernels, cap):
         assert (out.float() - plain.float()).abs().max() <= 2 ** -8
     else:
         check(kernels, q, kc, vc, bt, chunks, cap)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(24, 8, 128), (14, 2, 64), (12, 2, 128), (40, 1, 128)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_results_do_not_depend_on_what_ran_before(kernels, hq, hkv, d, cap):
+    """Groups that do not divide 128 leave rows of a query tile unused: their leftovers (infinite, tiny, NaN) change nothing."""
+    chunks = [(0, 300), (77, 130)]
+    q, kc, vc, bt = make(chunks, hq, hkv, d, 16, torch.bfloat16, gain=2.0)
+    full = make([(0, 2600)], 32, 8, d, 16, torch.bfloat16, seed=1)
+    want = check(kernels, q, kc, vc, bt, chunks, cap)
+    out, junk = torch.empty_like(q), torch.empty_like(full[0])
+    for leftover in (float("inf"), 1e30, 0.0, float("nan")):
+        full[0].fill_(leftover)                                  # every row of every query tile of this launch
+        call(kernels, junk, *full, [(0, 2600)], d ** -0.5, score_cap=cap)
+        call(kernels, out, q, kc, vc, bt, chunks, d ** -0.5, score_cap=cap)
+        assert torch.equal(out, want)

@@ -219,3 +219,15 @@ def test_the_largest_batches(kernels):
     call(kernels, out, *state)
     kernels.paged_attention_forward(plain, q, kc, vc, bt, sl, 0.125, 16, bt.size(1))
     assert (out.float() - plain.float()).abs().max() <= 2 ** -9
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 256), (32, 8, 128), (16, 16, 64)])
+def test_prefixes_that_end_inside_a_tile_many_pieces_to_a_cta(kernels, hq, hkv, d):
+    """Eleven groups whose prefixes end inside a key tile; few CTAs, so that one works through many pieces."""
+    groups = [(2000 + 16 * (3 * i % 8) + 64 * i, [1 + (7 * i + j) % 90 for j in range(9 + i)]) for i in range(11)]
+    state = make(groups, hq, hkv, d, 16, torch.bfloat16)
+    first = check(kernels, state)
+    few = check(kernels, state, max_ctas=5)
+    for _ in range(10):
+        assert torch.equal(check(kernels, state), first)
+        assert torch.equal(check(kernels, state, max_ctas=5), few)
