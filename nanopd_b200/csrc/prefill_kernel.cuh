@@ -51,7 +51,11 @@ using namespace npd;
 
 constexpr int kMaxChunks = 64;     // chunks per launch (kernel-parameter arrays)
 constexpr int kMaxPairs = 2048;    // query-tile pairs per launch (kernel-parameter array, heaviest first)
-constexpr int kSchedSlots = 4;     // work items the producer may publish ahead of the slowest consumer
+// Slots of the ring in which the producer publishes work items.  With items of a single key tile it publishes item n when
+// tile n - 1 has been requested, so when the scores of item n - 4 are complete (a ring of three K tiles), so when the PV
+// product of item n - 5 has been issued, which waits until the epilogue has taken item n - 6's accumulator out of TMEM.  The
+// epilogue may then still be writing that item's rows, with the slots of items n - 5 .. n yet to read: six.
+constexpr int kSchedSlots = 8;
 constexpr int kRows = 128;         // UMMA M: rows of one query tile
 constexpr int kKeys = 128;         // keys per K/V tile in shared memory (64 at head_dim 256)
 constexpr int kHalfKeys = 64;      // keys per half-step (UMMA N of a score MMA, K extent of a PV MMA batch)
@@ -611,8 +615,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         }
         for (int k = 0; ok; ++k) {
             // Warp 8 fetches and publishes the next work item; warp 11 reads it like the other roles.  A slot is
-            // reused kSchedSlots items later; by then every role has long read it (warp 8 cannot run more than
-            // two items ahead of the MMA warps, which cannot run ahead of the V tiles or the softmax groups).
+            // reused kSchedSlots items later; by then every role has read it (see there).
             int item = 0;
             ItemT it;
             if (MODE == kPrefix && k_role) {
@@ -1239,6 +1242,8 @@ int prepare_launch(const PrefillCall &c, int64_t total_tokens, PrefillLaunch &l)
     l.tile_keys = c.head_dim == 256 ? 64 : kKeys;
     l.smem = 1024 + l.query_tiles * halves * kQHalfBytes + (size_t)(kStagesK + kStagesV) * halves * l.tile_keys * 128 +
              sizeof(SmemCtrl) + 64;
+    static_assert(1024 + 2 * TileBytes<128>::q + (kStagesK + kStagesV) * TileBytes<128>::kv + sizeof(SmemCtrl) + 64 <= npd::kMaxDynamicSmem,
+                  "shared memory of a CTA");
     const bool f16 = c.dtype == NPD_DTYPE_F16;
 #define NPD_PICK_B(D_, B_) (f16 ? paged_prefill_kernel<__half, D_, B_, MODE> : paged_prefill_kernel<__nv_bfloat16, D_, B_, MODE>)
 #define NPD_PICK(D_) l.kernel = l.box_rows == 4 ? NPD_PICK_B(D_, 4) : (l.box_rows == 8 ? NPD_PICK_B(D_, 8) : NPD_PICK_B(D_, 16))

@@ -357,3 +357,30 @@ def test_partial_last_tiles_one_item_after_another(kernels, hq, hkv, d, max_ctas
         exact, A, l = shaped_oracle.attend(q[offs[i]:offs[i] + n], kc, vc, bt[i], s, d ** -0.5)
         tol = shaped_oracle.attention_tolerance(exact, A, l, s + n, q.dtype, 6.0)
         assert ((want[offs[i]:offs[i] + n].double() - exact).abs() <= tol).all(), f"chunk {i}"
+
+
+def test_hundreds_of_prompts_of_a_single_key_tile(kernels):
+    """Short prompts, one key tile each, on few CTAs: the producer runs as far ahead of the epilogue as it can."""
+    hq, hkv, d, block = 64, 8, 128, 16
+    chunks = [(0, 16 + i % 100) for i in range(60)]
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(5)
+    need = [-(-n // block) for _, n in chunks]
+    kc, vc = (torch.randn(sum(need), hkv, block, d, generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+    bt = torch.zeros(len(chunks), max(need), dtype=torch.int32, device=DEV)
+    at, offs = 0, []
+    for i, (_, n) in enumerate(chunks):
+        bt[i, :need[i]] = torch.arange(at, at + need[i], device=DEV)
+        at += need[i]
+        offs.append(sum(m for _, m in chunks[:i]))
+    q = torch.randn(sum(n for _, n in chunks), hq, d, generator=gen, device=DEV).to(torch.bfloat16)
+    args = (kc, vc, bt, offs, [n for _, n in chunks], [0] * len(chunks), d ** -0.5, block, bt.size(1))
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    kernels.paged_prefill_attention(want, q, *args)
+    for i in range(20):
+        kernels.paged_prefill_attention(out, q, *args, max_ctas=(1, 3, 20, 0)[i % 4])
+        assert torch.equal(out, want)
+    for i in (0, 17, 59):
+        n = chunks[i][1]
+        exact, A, l = shaped_oracle.attend(q[offs[i]:offs[i] + n], kc, vc, bt[i], 0, d ** -0.5)
+        assert ((want[offs[i]:offs[i] + n].double() - exact).abs() <= shaped_oracle.attention_tolerance(exact, A, l, n, q.dtype, 6.0)).all()

@@ -235,3 +235,16 @@ def test_results_do_not_depend_on_what_ran_before(kernels, hq, hkv, d, cap):
         call(kernels, junk, *full, [(0, 2600)], d ** -0.5, score_cap=cap)
         call(kernels, out, q, kc, vc, bt, chunks, d ** -0.5, score_cap=cap)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("hq,hkv,d,block", [(64, 8, 128, 8), (32, 1, 128, 16), (8, 8, 64, 16), (16, 2, 256, 16)])
+def test_many_items_of_a_single_key_tile(kernels, hq, hkv, d, block):
+    """A short window makes every work item one key tile long: the producer runs as far ahead of the epilogue as it can."""
+    chunks = [(0, 2775)]
+    q, kc, vc, bt = make(chunks, hq, hkv, d, block, torch.bfloat16, gain=0.3)
+    poison(kc, vc, bt, chunks, 6)
+    want = check(kernels, q, kc, vc, bt, chunks, 50.0, slopes_for(hq), 6)
+    out = torch.empty_like(q)
+    for i in range(40):
+        call(kernels, out, q, kc, vc, bt, chunks, d ** -0.5, score_cap=50.0, distance_slopes=slopes_for(hq), window=6, max_ctas=(0, 1, 5, 100)[i % 4])
+        assert torch.equal(out, want)
