@@ -290,3 +290,11 @@ def test_workspaces_are_dropped_and_made_again(kernels):
     from nanopd_b200 import paged_kernels
     paged_kernels.release_workspaces(DEV)
     assert torch.equal(check(kernels, q, kc, vc, bt, sl, scale, 50.0, max_ctas=140), want)
+
+
+@pytest.mark.parametrize("window", [0, 100000])
+def test_very_long_contexts(kernels, window):
+    lens = [150001, 7, 99999]
+    q, kc, vc, bt, sl, scale = make(lens, 4, 1, 128, 16, torch.bfloat16, gain=2.0)
+    check(kernels, q, kc, vc, bt, sl, scale, 30.0, None, window)
+    check(kernels, q, kc, vc, bt, sl, scale, 0.0, slopes_for(4) * 0.01, window)

@@ -231,3 +231,12 @@ def test_prefixes_that_end_inside_a_tile_many_pieces_to_a_cta(kernels, hq, hkv, 
     for _ in range(10):
         assert torch.equal(check(kernels, state), first)
         assert torch.equal(check(kernels, state, max_ctas=5), few)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 128), (12, 1, 64), (4, 1, 256)])
+def test_a_long_prefix_in_more_pieces_than_a_warp_has_lanes(kernels, hq, hkv, d):
+    """One item whose key tiles go to every SM: a row is joined from more than a hundred pieces."""
+    state = make([(30000, [5, 100, 1, 33, 64, 17, 2, 300])], hq, hkv, d, 16, torch.float16)
+    first = check(kernels, state)
+    assert torch.equal(check(kernels, state), first)
+    check(kernels, state, max_ctas=40)
