@@ -1459,9 +1459,6 @@ int run_decode(const DecodeCall &c) {
     NPD_CUDA_TRY(cudaGetDevice(&dev));
     LaunchShape ls = launch_shape(static_cast<int>(c.head_dim), static_cast<int>(c.block_size), (c.flags >> 8) & 0xffff,
                                   (long long)c.num_seqs * c.num_kv_heads, dev);
-    // The shaping of a tile's scores and the joining of pieces lengthen a warp's chain per tile: where plain scores take 8
-    // warps, these take 12 (256 ragged sequences, capped: 241 us against 248; behind 8192 shared tokens: 128 against 131)
-    if (MODE != kPlain && c.head_dim == 128 && ls.nstages == 2 && ls.nwarps == 8) ls.nwarps = NPD_DECODE_MAX_WARPS;
     const WorkspacePlan wp = plan_workspace(c.num_seqs, c.num_q_heads, c.num_kv_heads, c.head_dim, ls);
     NPD_REQUIRE(c.workspace != nullptr && c.workspace_bytes >= wp.total, NPD_ERR_WORKSPACE,
                 "decode attention: workspace of %zu bytes given, %zu needed", c.workspace_bytes, wp.total);
@@ -1537,7 +1534,9 @@ int run_decode(const DecodeCall &c) {
     p.block_shift = p.box_shift = 2;
     while (1 << p.block_shift < p.block_size) ++p.block_shift;
     while (1 << p.box_shift < p.box_rows) ++p.box_shift;
-    p.seg_cost = MODE == kTail ? 6 : 2;
+    // 256 sequences with 23 tiles of their own behind 8192 shared tokens: 126 us at a cost of 4, 122 at 8, 131 at 12; 256
+    // ragged sequences of 84 tiles: 220 us at 1 or 2, 221 at 4
+    p.seg_cost = MODE == kTail ? 8 : 2;
     p.cluster = ls.cluster;
     p.group_offsets = c.group_offsets;
     p.shared_lens = c.shared_lens;

@@ -1043,7 +1043,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                         for (int i = 0; i < 16; ++i) {
                             const float2 xs = exponents(make_float2(sc[cc][2 * i], sc[cc][2 * i + 1]));
                             // a cap already fills the FMA pipes: all exponentials on the special-function unit
-                            // (chunks of 512 tokens: 363 us; a quarter of them on the FMA pipes 380, an eighth 368)
+                            // (chunks of 512 tokens, when it was chosen: 363 us; a quarter of them on the FMA pipes 380, an eighth 368)
                             constexpr int kEvery = MODE == kCapped ? 0 : kPolyExpEvery;
                             const float2 pr = (kEvery > 0 && i % (kEvery > 0 ? kEvery : 1) == 0)
                                                   ? exp2_fma2(xs)
