@@ -51,11 +51,17 @@ using namespace npd;
 
 constexpr int kMaxChunks = 64;     // chunks per launch (kernel-parameter arrays)
 constexpr int kMaxPairs = 2048;    // query-tile pairs per launch (kernel-parameter array, heaviest first)
-// Slots of the ring in which the producer publishes work items.  With items of a single key tile it publishes item n when
-// tile n - 1 has been requested, so when the scores of item n - 4 are complete (a ring of three K tiles), so when the PV
-// product of item n - 5 has been issued, which waits until the epilogue has taken item n - 6's accumulator out of TMEM.  The
-// epilogue may then still be writing that item's rows, with the slots of items n - 5 .. n yet to read: six.
+// Slots of the ring in which the producer publishes work items.  Eight let it run as far ahead as the other rings allow: with
+// items of a single key tile it publishes item n when tile n - 1 has been requested, so when the scores of item n - 4 are
+// complete (a ring of three K tiles), so when the PV product of item n - 5 has been issued, which waits until the epilogue has
+// taken item n - 6's accumulator out of TMEM.  The epilogue may then still be writing that item's rows, with the slots of items
+// n - 5 .. n yet to read: six.  That the slot is free is not left to this: a softmax group without work in an item (the second
+// one of every single-tile item, of all items at head size 256) arrives on no other barrier, so every role says when it has
+// read a slot, and the producer waits for all of them before it publishes there again.
 constexpr int kSchedSlots = 8;
+// Arrivals that free a slot: every thread of the softmax and epilogue warps for itself (they leave one by one when a wait gives
+// up, so nothing here may wait for a whole warp), one per MMA warp and one of the V producer.
+constexpr int kSchedReaders = 12 * 32 + 3;
 constexpr int kRows = 128;         // UMMA M: rows of one query tile
 constexpr int kKeys = 128;         // keys per K/V tile in shared memory (64 at head_dim 256)
 constexpr int kHalfKeys = 64;      // keys per half-step (UMMA N of a score MMA, K extent of a PV MMA batch)
@@ -387,6 +393,7 @@ template <int MODE> __device__ __forceinline__ int item_t0(const typename ItemOf
 template <typename ItemT>
 struct alignas(8) SmemCtrlT {
     uint64_t sched_full[kSchedSlots];   // the producer warp has published the next work item
+    uint64_t sched_read[kSchedSlots];   // the other roles have read it (kSchedReaders arrivals)
     int sched_item[kSchedSlots];
     ItemT sched_desc[kSchedSlots];      // the published item, decoded once by the producer warp: the other roles'
                                         // way from one item to the next stays a few loads (their decoding it
@@ -528,9 +535,18 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         ok_ref = wait_or_abort(smem_u32(&ctrl->sched_full[slot]), (k / kSchedSlots) & 1, &ctrl->abort_flag, p.status);
         return ok_ref ? *reinterpret_cast<volatile int *>(&ctrl->sched_item[slot]) : -1;
     };
+    // Behind the copy of the k-th item: by a whole warp (MMA warps, V producer), or by every thread for itself.
+    auto item_read_by_warp = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctrl->sched_read[k % kSchedSlots]));
+    };
+    auto item_read = [&](int k) { mbar_arrive(smem_u32(&ctrl->sched_read[k % kSchedSlots])); };
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kSchedSlots; ++i) mbar_init(smem_u32(&ctrl->sched_full[i]), 1);
+        for (int i = 0; i < kSchedSlots; ++i) {
+            mbar_init(smem_u32(&ctrl->sched_full[i]), 1);
+            mbar_init(smem_u32(&ctrl->sched_read[i]), kSchedReaders);
+        }
         for (int i = 0; i < kStagesK; ++i) {
             mbar_init(smem_u32(&ctrl->k_full[i]), 1);
             mbar_init(smem_u32(&ctrl->k_empty[i]), 2);
@@ -614,8 +630,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             run.left = min(p.plan->units_per_worker, p.plan->total_units - static_cast<int>(blockIdx.x) * p.plan->units_per_worker);
         }
         for (int k = 0; ok; ++k) {
-            // Warp 8 fetches and publishes the next work item; warp 11 reads it like the other roles.  A slot is
-            // reused kSchedSlots items later; by then every role has read it (see there).
+            // Warp 8 fetches and publishes the next work item; warp 11 reads it like the other roles.
             int item = 0;
             ItemT it;
             if (MODE == kPrefix && k_role) {
@@ -634,6 +649,10 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             }
             if (k_role) {
                 if (MODE != kPrefix && item >= 0) it = decode_item<MODE>(p, item);
+                if (k >= kSchedSlots) {                         // the slot's last item has been read by everyone
+                    ok = wait_or_abort(smem_u32(&ctrl->sched_read[k % kSchedSlots]), (k / kSchedSlots - 1) & 1, abort_flag, p.status);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                }
                 if (lane == 0) {
                     if (item >= 0) ctrl->sched_desc[k % kSchedSlots] = it;
                     *reinterpret_cast<volatile int *>(&ctrl->sched_item[k % kSchedSlots]) = item;
@@ -643,6 +662,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             } else {
                 if (item < 0) break;
                 it = ctrl->sched_desc[k % kSchedSlots];
+                item_read_by_warp(k);
             }
             const int32_t *table = p.block_tables + (long long)it.c * p.bt_row_stride;
             // A box lies in one block: 16 keys of a block of 16 or 32, or all keys of a block of 8 or 4.
@@ -809,6 +829,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const int item = next_item(k, ok);
                 if (!__all_sync(0xffffffffu, ok) || item < 0) break;
                 const ItemT it = ctrl->sched_desc[k % kSchedSlots];
+                item_read_by_warp(k);
                 const int U = it.nhalf[x], my_tiles = it.ntiles[x];
                 if (U > 0 && q_item < k) {
                     if (request_q(it, true) < 0) {
@@ -888,6 +909,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
             const ItemT it = ctrl->sched_desc[k % kSchedSlots];
+            item_read(k);
 #pragma unroll
             for (int x = 0; x < kQueryTiles; ++x) {
                 const int U = it.nhalf[x];
@@ -971,6 +993,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
             const ItemT it = ctrl->sched_desc[k % kSchedSlots];
+            item_read(k);
             const int U = x == 0 ? it.nhalf[0] : it.nhalf[1];
             const int t0 = item_t0<MODE>(it);
             const int first_pos = it.start + (x == 0 ? it.tok0[0] : it.tok0[1]);       // of the tile's first row

@@ -1,0 +1,73 @@
+"""CPU: the ring of published work items of the prompt kernel, as its source has it.
+
+A model of the ring under an adversarial order of steps: one producer that publishes items into slots, readers that wait for a
+slot's phase by its parity, as an mbarrier wait does (a parity tells a phase from the next one, not from the one after that).
+Readers may be held up for as long as nothing in the kernel waits for them."""
+import random
+import re
+from pathlib import Path
+
+import pytest
+
+SOURCE = (Path(__file__).resolve().parents[1] / "nanopd_b200" / "csrc" / "prefill_kernel.cuh").read_text()
+SLOTS = int(re.search(r"constexpr int kSchedSlots = (\d+);", SOURCE).group(1))
+
+
+def run(items, readers, waits_for_readers, pick):
+    """True when every reader has seen every item in order; False when one takes a later item for the awaited one or can
+    make no further step."""
+    published, slots, read = 0, [None] * SLOTS, [0] * readers
+    while True:
+        able = []
+        if published < items:
+            # the producer's wait: everyone has read what the slot held
+            if not waits_for_readers or published < SLOTS or min(read) > published - SLOTS:
+                able.append(-1)
+        for r in range(readers):
+            k = read[r]
+            if k < items:
+                phases = (published - k % SLOTS + SLOTS - 1) // SLOTS         # completed phases of slot k % SLOTS
+                if phases > 0 and (phases - 1) % 2 == (k // SLOTS) % 2:
+                    able.append(r)
+        if not able:
+            return published == items and all(k == items for k in read)
+        step = pick(able)
+        if step == -1:
+            slots[published % SLOTS] = published
+            published += 1
+        else:
+            if slots[read[step] % SLOTS] != read[step]:
+                return False
+            read[step] += 1
+
+
+def late(able):
+    """The reader 0 moves only when nobody else can."""
+    others = [a for a in able if a != 0]
+    return others[0] if others else 0
+
+
+def test_a_reader_that_nobody_waits_for_loses_the_ring():
+    assert not run(5 * SLOTS, 3, False, late)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_the_producer_waits_for_every_reader(seed):
+    assert run(5 * SLOTS, 3, True, late)
+    rng = random.Random(seed)
+    assert run(7 * SLOTS + 3, 4, True, rng.choice)
+
+
+def test_the_kernel_has_that_wait():
+    """The producer waits for the slot's readers before it writes there, and every role that copies an item arrives behind the
+    copy, as often as the barrier expects."""
+    wait = SOURCE.index("wait_or_abort(smem_u32(&ctrl->sched_read[k % kSchedSlots]), (k / kSchedSlots - 1) & 1")
+    assert wait < SOURCE.index("ctrl->sched_desc[k % kSchedSlots] = it;")
+    assert "if (k >= kSchedSlots)" in SOURCE[wait - 200:wait]
+    assert "mbar_init(smem_u32(&ctrl->sched_read[i]), kSchedReaders)" in SOURCE
+    copies = [m.end() for m in re.finditer(r"\bit = ctrl->sched_desc\[k % kSchedSlots\];", SOURCE)]
+    after = [SOURCE[c:c + 60].split()[0] for c in copies]
+    # V producer, MMA warps (two run that code), epilogue, softmax
+    assert after == ["item_read_by_warp(k);", "item_read_by_warp(k);", "item_read(k);", "item_read(k);"]
+    readers = re.search(r"constexpr int kSchedReaders = (\d+) \* 32 \+ (\d+);", SOURCE)
+    assert (int(readers.group(1)), int(readers.group(2))) == (4 + 8, 1 + 2)
