@@ -713,7 +713,10 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
 
     uint8_t *stage_base = sbase + (size_t)warp * nst * STAGE_BYTES;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sbase + (size_t)nwarps * nst * STAGE_BYTES) + warp * nst;
-    int *pre = reinterpret_cast<int *>(sbase + (size_t)nwarps * nst * (STAGE_BYTES + 8));
+    // kTail: the rows' scratch behind the prefix is read in 16-byte pieces, so the barriers are padded to such a piece (an odd
+    // number of stages an SM, which the tuning knobs allow, ends in the middle of one)
+    const size_t bar_bytes = MODE == kTail ? ((size_t)nwarps * nst * 8 + 15) / 16 * 16 : (size_t)nwarps * nst * 8;
+    int *pre = reinterpret_cast<int *>(sbase + (size_t)nwarps * nst * STAGE_BYTES + bar_bytes);
     float *scratch = nullptr;        // kTail: this warp's rows on their way out; a cluster: the CTA's record
     if (SMALL && MODE == kScored) scratch = reinterpret_cast<float *>(pre + 4);
     if (MODE == kTail)
@@ -1265,6 +1268,7 @@ int choose_kv_rep(int group, int max_heads) {
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 constexpr int kDecodeMaxSmem = npd::kMaxDynamicSmem - 1024;      // the kernel has some static shared memory too
+// (32 bytes: the barriers' padding, and the prefix rounded up to four words)
 size_t tail_smem(int head_dim, int group, const LaunchShape &ls, int64_t num_seqs) {
     const size_t stage_bytes = 2 * kTile * (size_t)head_dim * 2;
     return 1024 + (size_t)ls.nwarps * ls.nstages * (stage_bytes + 8) + ((size_t)num_seqs + 1) * 4 + 32 +
