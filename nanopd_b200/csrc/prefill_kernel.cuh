@@ -55,13 +55,13 @@ constexpr int kMaxPairs = 2048;    // query-tile pairs per launch (kernel-parame
 // items of a single key tile it publishes item n when tile n - 1 has been requested, so when the scores of item n - 4 are
 // complete (a ring of three K tiles), so when the PV product of item n - 5 has been issued, which waits until the epilogue has
 // taken item n - 6's accumulator out of TMEM.  The epilogue may then still be writing that item's rows, with the slots of items
-// n - 5 .. n yet to read: six.  That the slot is free is not left to this: a softmax group without work in an item (the second
-// one of every single-tile item, of all items at head size 256) arrives on no other barrier, so every role says when it has
-// read a slot, and the producer waits for all of them before it publishes there again.
+// n - 5 .. n yet to read: six.  The first softmax group, the MMA warps and the V producer take part in those steps and have read
+// item n - 5; the second softmax group arrives nowhere for an item in which its query tile has no work (every single-tile
+// item, all of them at head size 256), so it says when it is through with a slot, and the producer waits for that before it
+// publishes there again.
 constexpr int kSchedSlots = 8;
-// Arrivals that free a slot: every thread of the softmax and epilogue warps for itself (they leave one by one when a wait gives
-// up, so nothing here may wait for a whole warp), one per MMA warp and one of the V producer.
-constexpr int kSchedReaders = 12 * 32 + 3;
+constexpr int kSchedReaders = 128; // arrivals that free a slot: each thread of the second softmax group for itself (threads
+                                   // leave one by one when a wait gives up, so nothing here may wait for a whole warp)
 constexpr int kRows = 128;         // UMMA M: rows of one query tile
 constexpr int kKeys = 128;         // keys per K/V tile in shared memory (64 at head_dim 256)
 constexpr int kHalfKeys = 64;      // keys per half-step (UMMA N of a score MMA, K extent of a PV MMA batch)
@@ -393,7 +393,7 @@ template <int MODE> __device__ __forceinline__ int item_t0(const typename ItemOf
 template <typename ItemT>
 struct alignas(8) SmemCtrlT {
     uint64_t sched_full[kSchedSlots];   // the producer warp has published the next work item
-    uint64_t sched_read[kSchedSlots];   // the other roles have read it (kSchedReaders arrivals)
+    uint64_t sched_read[kSchedSlots];   // the second softmax group is through with it (kSchedReaders arrivals)
     int sched_item[kSchedSlots];
     ItemT sched_desc[kSchedSlots];      // the published item, decoded once by the producer warp: the other roles'
                                         // way from one item to the next stays a few loads (their decoding it
@@ -535,12 +535,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         ok_ref = wait_or_abort(smem_u32(&ctrl->sched_full[slot]), (k / kSchedSlots) & 1, &ctrl->abort_flag, p.status);
         return ok_ref ? *reinterpret_cast<volatile int *>(&ctrl->sched_item[slot]) : -1;
     };
-    // Behind the copy of the k-th item: by a whole warp (MMA warps, V producer), or by every thread for itself.
-    auto item_read_by_warp = [&](int k) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctrl->sched_read[k % kSchedSlots]));
-    };
-    auto item_read = [&](int k) { mbar_arrive(smem_u32(&ctrl->sched_read[k % kSchedSlots])); };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSchedSlots; ++i) {
@@ -649,7 +643,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             }
             if (k_role) {
                 if (MODE != kPrefix && item >= 0) it = decode_item<MODE>(p, item);
-                if (k >= kSchedSlots) {                         // the slot's last item has been read by everyone
+                if (k >= kSchedSlots) {                         // the slot's last item has been read
                     ok = wait_or_abort(smem_u32(&ctrl->sched_read[k % kSchedSlots]), (k / kSchedSlots - 1) & 1, abort_flag, p.status);
                     if (!__all_sync(0xffffffffu, ok)) break;
                 }
@@ -662,7 +656,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             } else {
                 if (item < 0) break;
                 it = ctrl->sched_desc[k % kSchedSlots];
-                item_read_by_warp(k);
             }
             const int32_t *table = p.block_tables + (long long)it.c * p.bt_row_stride;
             // A box lies in one block: 16 keys of a block of 16 or 32, or all keys of a block of 8 or 4.
@@ -829,7 +822,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const int item = next_item(k, ok);
                 if (!__all_sync(0xffffffffu, ok) || item < 0) break;
                 const ItemT it = ctrl->sched_desc[k % kSchedSlots];
-                item_read_by_warp(k);
                 const int U = it.nhalf[x], my_tiles = it.ntiles[x];
                 if (U > 0 && q_item < k) {
                     if (request_q(it, true) < 0) {
@@ -863,7 +855,32 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                     const int cu = c + u, buf = cu & 1;
                     // O_X is overwritten by the first PV of an item: the previous epilogue must have read it
                     if (u == 0 && items_done > 0 && !(ok = wait_all(&ctrl->o_free[x], (items_done - 1) & 1))) break;
-                    if (h == 0 && !(ok = wait_all(&ctrl->v_full[stage], (gt / kStagesV) & 1))) break;
+                    if (h == 0) {
+                        if (!(ok = wait_all(&ctrl->v_full[stage], (gt / kStagesV) & 1))) break;
+                        // V rows that no row of the item may see — at or past ctx_end, never written or never loaded; before
+                        // the item's window, not loaded or no longer its own — may hold anything: clear them, so that P = 0
+                        // there cannot meet a NaN.  Each MMA warp does it for its own products (twice the same zeros), here
+                        // where it has waited for the tile anyway: beside the softmax of the half-step, and off the softmax
+                        // warps, whose loop is 7 % slower with this branch in it.
+                        const int tile_key0 = (item_t0<MODE>(it) + t) * kTK, behind_from = it.ctx_end - tile_key0;
+                        int before_to = 0;
+                        if constexpr (shapes(MODE)) before_to = it.lo - tile_key0;
+                        if (behind_from < kTK || before_to > 0) {
+                            uint8_t *v_tile = v_ring + (size_t)stage * kKvTileBytes;
+                            constexpr int kPieces = kHalves * 8;           // 16-byte pieces per row
+                            auto clear = [&](int first, int last) {
+                                for (int idx = lane; idx < (last - first) * kPieces; idx += 32) {
+                                    const int r = first + idx / kPieces, piece = idx % kPieces;
+                                    *reinterpret_cast<uint4 *>(v_tile + (piece >> 3) * kKvHalfBytes + r * 128 + ((piece & 7) << 4)) =
+                                        make_uint4(0, 0, 0, 0);
+                                }
+                            };
+                            if (before_to > 0) clear(0, before_to);
+                            if (behind_from < kTK) clear(behind_from, kTK);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                    }
                     NPD_TRACE(x == 0 ? 1 : 4, 10, u);
                     if (!(ok = wait_all(&ctrl->p_ready[x][buf], (cu >> 1) & 1))) break;
                     NPD_TRACE(x == 0 ? 1 : 4, 11, u);
@@ -909,7 +926,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
             const ItemT it = ctrl->sched_desc[k % kSchedSlots];
-            item_read(k);
 #pragma unroll
             for (int x = 0; x < kQueryTiles; ++x) {
                 const int U = it.nhalf[x];
@@ -982,7 +998,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
         const uint32_t t_sx = tmem + x * 128 + lane_base;        // two score buffers of 64 columns
         const uint32_t t_o = tmem + 256 + x * 128 + lane_base;
         const int tq_idx = row / p.group, hg = row - tq_idx * p.group;
-        int g = 0, c = 0;                                     // key tiles / own half-steps so far (barrier phases)
+        int c = 0;                                            // own half-steps so far (barrier phases)
         int items_handed = 0;                                 // items handed to the epilogue warps so far
         const int sm_role = wq == 0 ? 2 + x : 5 + x * 3 + (wq - 1);   // trace slot (used only by tracing builds)
         (void)sm_role;
@@ -993,7 +1009,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
             const int item = next_item(k, ok);
             if (!ok || item < 0) break;
             const ItemT it = ctrl->sched_desc[k % kSchedSlots];
-            item_read(k);
             const int U = x == 0 ? it.nhalf[0] : it.nhalf[1];
             const int t0 = item_t0<MODE>(it);
             const int first_pos = it.start + (x == 0 ? it.tok0[0] : it.tok0[1]);       // of the tile's first row
@@ -1009,7 +1024,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
 #pragma unroll 1
             for (int u = 0; ok && u < U; ++u) {
                 const int cu = c + u, buf = cu & 1;
-                const int t = u / kHPT, gt = g + t, stage = gt % kStagesV;
                 const int key0 = t0 * kTK + u * kHalfKeys;
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 20, u);
                 if (!(ok = wait_or_abort(smem_u32(&ctrl->s_full[x][buf]), (cu >> 1) & 1, abort_flag, p.status))) break;
@@ -1141,34 +1155,6 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                     probabilities([&](float2 y) { return __ffma2_rn(y, scale2, negm2); });
                 }
                 if (lane == 0) NPD_TRACE_FINE(sm_role, 24, u);
-                // V rows that no row of the item may see — at or past ctx_end, never written or never loaded; before the item's
-                // window, not loaded or no longer its own — may hold anything: clear them, so that P = 0 there cannot meet a
-                // NaN.  Both softmax groups do it (idempotent), at the first half-step of the key tile, before they release
-                // its probabilities.  Only here, behind the wait for the half-step's scores: a parity wait for a ring stage is
-                // sound once the stage's tile before has landed, and these groups wait for V tiles nowhere else.  The MMA warp
-                // that issued the scores had waited for that tile — for every tile of the items before, also of those this
-                // query tile had no part in, and for the tiles of the PV products it had issued, this half-step's last but two
-                // among them.
-                if (u % kHPT == 0) {
-                    const int tile_key0 = key0, behind_from = max(0, it.ctx_end - tile_key0);
-                    int before_to = 0;
-                    if constexpr (shapes(MODE)) before_to = u == 0 ? max(0, it.lo - tile_key0) : 0;
-                    if (behind_from < kTK || before_to > 0) {
-                        if (!(ok = wait_or_abort(smem_u32(&ctrl->v_full[stage]), (gt / kStagesV) & 1, abort_flag, p.status))) break;
-                        uint8_t *v_tile = v_ring + (size_t)stage * kKvTileBytes;
-                        constexpr int kPieces = kHalves * 8;           // 16-byte pieces per row
-                        auto clear = [&](int first, int last) {
-                            for (int idx = threadIdx.x & 127; idx < (last - first) * kPieces; idx += 128) {
-                                const int r = first + idx / kPieces, piece = idx % kPieces;
-                                *reinterpret_cast<uint4 *>(v_tile + (piece >> 3) * kKvHalfBytes + r * 128 + ((piece & 7) << 4)) =
-                                    make_uint4(0, 0, 0, 0);
-                            }
-                        };
-                        if (before_to > 0) clear(0, before_to);
-                        if (behind_from < kTK) clear(behind_from, kTK);
-                        fence_proxy_async_smem();
-                    }
-                }
                 tmem_wait_st();
                 tc_fence_before();           // P is in TMEM, S has been read: the MMA warp may go on
                 mbar_arrive(smem_u32(&ctrl->p_ready[x][buf]));
@@ -1193,8 +1179,8 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 mbar_arrive(smem_u32(&ctrl->epi_ready[x]));
                 ++items_handed;
             }
+            if (x == 1) mbar_arrive(smem_u32(&ctrl->sched_read[k % kSchedSlots]));
             if (lane == 0) NPD_TRACE(sm_role, 32, k);
-            g += it.n_kv;
             c += U;
         }
     }
