@@ -283,7 +283,8 @@ int npd_paged_scored_prefill_attention(void *out, const void *q, const void *k_c
  * pages that several sequences share read and multiplied once per group of sequences.
  * Group g is the sequences group_offsets[g] <= s < group_offsets[g + 1] (device int32
  * [num_groups + 1], ascending); their first shared_lens[g] tokens (device int32 [num_groups])
- * lie in the same pages, that is, their table rows agree there.  Sequences outside every group,
+ * lie in the same pages, that is, the table rows of its sequences that are not empty agree there
+ * (the rows of empty sequences are not read).  Sequences outside every group,
  * groups of one, and what a shared_len reaches beyond the shortest non-empty sequence of its
  * group are attended to as in npd_paged_decode_attention.  Only whole tiles of 16 tokens are
  * shared; the rest of a prefix is read per sequence.  The lengths, offsets and tables are read on

@@ -474,7 +474,7 @@ __device__ __forceinline__ bool prefix_item(const PrefillParams &p, PrefixRun &r
     }
     const int tile_keys = kHalfKeys * p.half_steps_per_tile;
     const int n = min(g.key_tiles - run.at.tile, run.left);
-    it.c = g.begin;                                             // the first sequence's table row names the shared pages
+    it.c = g.table_seq;
     it.h = run.at.head;
     it.start = 0;
     it.qoff = g.begin;

@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     int *offs = plan_smem;                       // [num_groups + 1] group_offsets
     int *unit = offs + p.num_groups + 1;         // [num_groups + 1] units in front of each group
     int *least = unit + p.num_groups + 1;        // [num_groups] shortest sequence that is not empty
+    int *first = least + p.num_groups;           // [num_groups] first sequence that is not empty: an empty one's table row may
+                                                 // name anything (an idle slot's is parked on a page that nobody reads)
     __shared__ int bad;
     const int tid = threadIdx.x;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     if (tid == 0) bad = 0;
     for (int g = tid; g <= p.num_groups; g += blockDim.x) {
         offs[g] = p.group_offsets[g];
-        if (g < p.num_groups) least[g] = INT32_MAX;
+        if (g < p.num_groups) least[g] = first[g] = INT32_MAX;
     }
     __syncthreads();                             // `bad` and the offsets are set
     // Groups must be consecutive ranges of the batch.  Anything else shares nothing (every row is still right: the tail
@@ -95,11 +97,14 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
     for (int s = tid; s < p.num_seqs; s += blockDim.x) {
         const int n = s == tid ? my_len : p.seq_lens[s];
         const int g = group_of(s);
-        if (g >= 0 && n > 0) atomicMin(least + g, n);
+        if (g >= 0 && n > 0) {
+            atomicMin(least + g, n);
+            atomicMin(first + g, s);
+        }
     }
     __syncthreads();
     for (int g = tid; g < p.num_groups; g += blockDim.x) {
-        PrefixGroup out{0, 0, 0, 0};
+        PrefixGroup out{0, 0, 0, 0, 0};
         if (!none) {
             out.begin = offs[g];
             out.seqs = offs[g + 1] - offs[g];
@@ -109,6 +114,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
             if (out.seqs > 1 && least[g] != INT32_MAX) {
                 const long long most = min((long long)least[g], p.cap) - 1;
                 out.tokens = static_cast<int>(min((long long)max(shared, 0), most)) / kTile * kTile;
+                out.table_seq = first[g];
             }
             out.key_tiles = (out.tokens + p.tile_keys - 1) / p.tile_keys;
         }
@@ -245,7 +251,7 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
     pp.tile_keys = tile_keys;
     pp.workers = cap > 0 && cap < sms ? cap : sms;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    constexpr size_t plan_most = (size_t)(3 * kMaxGroups + 2) * sizeof(int);
+    constexpr size_t plan_most = (size_t)(4 * kMaxGroups + 2) * sizeof(int);
     static std::atomic<unsigned long long> plan_done{0};
     if (npd::first_on_device(plan_done, dev)) {
         NPD_CUDA_TRY(cudaFuncSetAttribute(shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_most));
@@ -253,7 +259,7 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
     }
     // a barrier of 1024 threads costs more than what a batch of a few hundred sequences gives them to do
     const int plan_threads = num_seqs <= 512 && num_groups <= 512 ? 256 : kPlanThreads;
-    shared_prefix_plan_kernel<<<1, plan_threads, (size_t)(3 * num_groups + 2) * sizeof(int), st>>>(pp);
+    shared_prefix_plan_kernel<<<1, plan_threads, (size_t)(4 * num_groups + 2) * sizeof(int), st>>>(pp);
     NPD_CUDA_TRY(cudaGetLastError());
     npd::PrefixPass pass{q, k_cache, v_cache, block_tables, scale, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
                          max_blocks_per_seq, num_blocks, cache_block_stride, bt_row_stride, dtype, status, pp.groups, pp.seeds,

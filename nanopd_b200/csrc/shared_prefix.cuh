@@ -21,6 +21,7 @@ struct PrefixGroup {
     int begin, seqs;      // sequences of the group
     int tokens;           // shared tokens that the prefix pass covers, a multiple of 16
     int key_tiles;        // K/V tiles of them
+    int table_seq;        // the group's first sequence that is not empty: its table row names the shared pages
 };
 struct PrefixSeed {
     int group, pair, head, tile;      // where a CTA's run of units begins

@@ -121,7 +121,8 @@ class SyntheticDecoder:
 
         ``group_offsets`` and ``shared_lens`` (int32 ``[groups + 1]`` and ``[groups]``) name the sequences whose tables begin
         with the same pages: layers whose scores are not shaped then attend with
-        ``paged_kernels.paged_shared_prefix_attention``.  They may be rewritten in place too."""
+        ``paged_kernels.paged_shared_prefix_attention``.  They may be rewritten in place too.  An idle slot of a group has
+        its own page in its row like any other idle slot."""
         s = self.shape
         if k_cache.dim() != 5 or k_cache.size(0) != s.num_layers or k_cache.size(2) != s.num_kv_heads or k_cache.size(4) != s.head_dim:
             raise RuntimeError("k_cache must be [num_layers, blocks, Hkv, B, D] for this decoder's shape")

@@ -655,7 +655,8 @@ def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tabl
     """:func:`paged_attention_forward` for a batch whose sequences share the first pages of their tables, written in place.
 
     Group ``g`` is the sequences ``group_offsets[g] <= s < group_offsets[g + 1]`` (int32 ``[groups + 1]`` on the device, ascending);
-    the first ``shared_lens[g]`` tokens (int32 ``[groups]``) of each lie in the same pages: their ``block_tables`` rows agree there.
+    the first ``shared_lens[g]`` tokens (int32 ``[groups]``) of each lie in the same pages: their ``block_tables`` rows agree there
+    (those of sequences of length 0 are not read).
     Those pages are read once per group, on the tensor cores, instead of once per sequence.  Sequences outside every group and
     groups of one are attended to as usual, and so is what ``shared_lens`` reaches beyond the shortest non-empty sequence of the
     group.  Lengths, offsets and tables are read on the device, so they may change between replays of a captured call; offsets

@@ -6,9 +6,31 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
+
+from test_gpu_shared_prefix import check, make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("idle", [(0,), (0, 1), (2,), (0, 3), (1, 2, 3)])
+@pytest.mark.parametrize("max_ctas", [0, 140])
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (12, 2, 64), (16, 2, 256)])
+def test_idle_slots_whose_rows_name_other_pages(kernels, hq, hkv, d, max_ctas, idle):
+    """An empty slot's table row is parked on a page of NaN (and, behind it, names no page at all): neither the group's other
+    sequences nor the status word see it."""
+    q, kc, vc, bt, sl, go, sh = make([(96, [5, 8]), (512, [9, 30, 100, 7]), (64, [3, 4])], hq, hkv, d, 16, torch.bfloat16)
+    used = set(bt[:, :].flatten().tolist())
+    parked = next(i for i in range(kc.size(0)) if i not in used or bool(torch.isnan(kc[i]).all()))
+    kc[parked], vc[parked] = float("nan"), float("nan")
+    for i in idle:
+        sl[2 + i] = 0
+        bt[2 + i] = -5
+        bt[2 + i, 0] = parked
+    out = check(kernels, (q, kc, vc, bt, sl, go, sh), max_ctas=max_ctas)
+    for i in idle:
+        assert (out[2 + i] == 0).all()
 
 
 def test_an_odd_number_of_stages_of_a_cta(kernels):
