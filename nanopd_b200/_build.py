@@ -19,7 +19,7 @@ LIB_PATH = PKG_DIR / "libnanopd_b200.so"
 SOURCES = ["capi.cu", "kv_store.cu", "decode_attention.cu", "prefill_attention.cu", "kv_migrate.cu",
            "qk_rope_store.cu", "top_k_sample.cu", "scored_attention.cu", "scored_prefill.cu",
            "shared_prefix.cu", "prefix_pass.cu", "residual_norms.cu", "packed.cu"]
-HEADERS = [CSRC / "npd_common.cuh", CSRC / "decode_kernel.cuh", CSRC / "prefill_kernel.cuh",
+HEADERS = [CSRC / "npd_common.cuh", CSRC / "capped_scores.cuh", CSRC / "decode_kernel.cuh", CSRC / "prefill_kernel.cuh",
            CSRC / "shared_prefix.cuh", PKG_DIR.parent / "include" / "nanopd_b200.h",
            PKG_DIR.parent / "include" / "nanopd_b200_testing.h"]
 NVCC_FLAGS = [

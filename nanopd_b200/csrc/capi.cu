@@ -84,7 +84,7 @@ int encode_cache_tensor_map(CUtensorMap *map, const void *base, int dtype, int64
 int check_score_shape(const char *op, float scale, float score_cap, const float *distance_slopes, int64_t window) {
     const float cap_in = score_cap > 0.f ? 2.f * 1.4426950408889634f * scale / score_cap : 0.f;
     NPD_REQUIRE(std::isfinite(scale) && scale >= 0.f, NPD_ERR_INVALID_ARG, "%s: the scale must be finite and not negative", op);
-    NPD_REQUIRE(std::isfinite(score_cap) && (score_cap == 0.f || score_cap >= 1e-30f) && std::isfinite(cap_in) && std::isfinite(score_cap * 1.5f),
+    NPD_REQUIRE(score_cap == 0.f || (score_cap >= 1e-30f && score_cap <= 1e38f && std::isfinite(cap_in)),
                 NPD_ERR_INVALID_ARG, "%s: the score cap must be 0 (none) or between 1e-30 and 1e38", op);
     NPD_REQUIRE(window >= 0, NPD_ERR_INVALID_ARG, "%s: the window must not be negative (0 = none)", op);
     NPD_REQUIRE((reinterpret_cast<uintptr_t>(distance_slopes) & 3u) == 0, NPD_ERR_INVALID_ARG,

@@ -33,6 +33,7 @@
 #include <atomic>
 #include <cstdlib>
 
+#include "capped_scores.cuh"
 #include "npd_common.cuh"
 #include "shared_prefix.cuh"
 
@@ -72,8 +73,7 @@ struct DecodeParams {
     int block_shift, box_shift;      // log2 of block_size and box_rows (kScored and kTail)
     int seg_cost;         // see unit_at; kScored and kTail
     // kScored: scores are shaped before the softmax (all in the log2 domain)
-    float cap_in;         // 2 log2(e) * scale / cap, the exponent's factor in tanh; 0 = scores are not capped
-    float cap_log2;       // cap * log2(e)
+    ScoreCap cap;
     const float *slopes;  // [num_q_heads] slope of the distance bias, or nullptr
     int window;           // keys visible behind the query, its own included; INT32_MAX = all
     int cluster;          // small form: CTAs that share a (sequence, virtual kv head)
@@ -532,12 +532,25 @@ __device__ __forceinline__ void merge_partials(AttnState<T, D, NT> &st, const De
     }
 }
 
-// A score of kScored in the log2 domain: scale, cap, distance bias.  tanh(z) = 1 - 2 / (1 + e^2z) loses digits near
-// z = 0 in relative terms only: its absolute error stays near 2^-23, that of the capped score near cap * 2^-23.
-__device__ __forceinline__ float shaped_score(float raw, float slope_log2, int key, int pos, const DecodeParams &p) {
-    float x = raw * p.scale_log2;
-    if (p.cap_in != 0.f) x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + fast_exp2(raw * p.cap_in)));
-    return x + slope_log2 * static_cast<float>(key - pos);
+// kScored: the raw scores of a tile's four (key, head) places of this thread, scaled and capped, in the log2 domain.  The
+// exponential and the reciprocal of scores near the cap are computed only where the warp has one.
+__device__ __forceinline__ void scale_and_cap(float (&x)[4], const DecodeParams &p) {
+    if (p.cap.in == 0.f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= p.scale_log2;
+        return;
+    }
+    const float2 a = make_float2(x[0], x[1]), b = make_float2(x[2], x[3]);
+    const float most = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
+    float2 ya, yb;
+    if (__any_sync(0xffffffffu, most >= p.cap.edge)) {
+        ya = capped_any(a, p.scale_log2, p.cap);
+        yb = capped_any(b, p.scale_log2, p.cap);
+    } else {
+        ya = capped_near(a, p.scale_log2, p.cap);
+        yb = capped_near(b, p.scale_log2, p.cap);
+    }
+    x[0] = ya.x, x[1] = ya.y, x[2] = yb.x, x[3] = yb.y;
 }
 
 // Floats of a warp's scratch for write_joined: `group` rows of D values (padded: the writes below are free of bank
@@ -1012,16 +1025,21 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
             const int key_a = tok0 + g, key_b = key_a + 8;
             const bool va = key_a < seg_len && (MODE != kScored || key_a >= seg_lo);
             const bool vb = key_b < seg_len && (MODE != kScored || key_b >= seg_lo);
-            auto score = [&](float raw, int key, int nt, int e) {
-                if (MODE == kScored) return shaped_score(raw, slope[nt][e], key, seg_len - 1, p);
-                return raw * p.scale_log2;
-            };
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float x0 = va ? score(sa[nt][0] + sb[nt][0], key_a, nt, 0) : -INFINITY;
-                const float x1 = va ? score(sa[nt][1] + sb[nt][1], key_a, nt, 1) : -INFINITY;
-                const float x2 = vb ? score(sa[nt][2] + sb[nt][2], key_b, nt, 0) : -INFINITY;
-                const float x3 = vb ? score(sa[nt][3] + sb[nt][3], key_b, nt, 1) : -INFINITY;
+                float x[4];                                  // (key_a, head 2t), (key_a, 2t+1), (key_b, 2t), (key_b, 2t+1)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = sa[nt][e] + sb[nt][e];
+                if (MODE == kScored) {
+                    scale_and_cap(x, p);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] += slope[nt][e & 1] * static_cast<float>((e < 2 ? key_a : key_b) - (seg_len - 1));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] *= p.scale_log2;
+                }
+                const float x0 = va ? x[0] : -INFINITY, x1 = va ? x[1] : -INFINITY;
+                const float x2 = vb ? x[2] : -INFINITY, x3 = vb ? x[3] : -INFINITY;
                 float mx0 = fmaxf(x0, x2), mx1 = fmaxf(x1, x3);
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
@@ -1531,8 +1549,7 @@ int run_decode(const DecodeCall &c) {
     p.bt_row_stride = c.bt_row_stride;
     p.num_workers = ls.grid * ls.nwarps;
     p.num_stages = ls.nstages;
-    p.cap_in = c.score_cap > 0.f ? 2.f * 1.4426950408889634f * c.scale / c.score_cap : 0.f;
-    p.cap_log2 = c.score_cap * 1.4426950408889634f;
+    p.cap = make_score_cap(c.scale, c.score_cap);
     p.slopes = c.slopes;
     p.window = c.window > 0 && c.window < INT32_MAX ? static_cast<int>(c.window) : INT32_MAX;
     p.block_shift = p.box_shift = 2;

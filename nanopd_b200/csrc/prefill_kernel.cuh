@@ -42,6 +42,7 @@
 #include <cmath>
 #include <vector>
 
+#include "capped_scores.cuh"
 #include "npd_common.cuh"
 #include "shared_prefix.cuh"
 
@@ -120,10 +121,9 @@ struct PrefillParams {
     int chunk_q_offset[kMaxChunks];
     int chunk_tokens[kMaxChunks];
     int chunk_start[kMaxChunks];
-    // kCapped: a capped score in the log2 domain is x Q(x^2), x = q . k, for |x| < cap_reach (Q: cap_poly), and
-    // cap_log2 - 2 cap_log2 / (1 + 2^(cap_in x)) elsewhere (tanh z = 1 - 2 / (1 + e^2z))
-    float cap_in;                     // 2 log2(e) * scale / cap
-    float cap_log2;                   // cap * log2(e)
+    // kCapped: half-steps without mask and bias whose scores x = q . k are all below cap_reach take x Q(x^2) (Q: cap_poly),
+    // see fill_shaping; the others go by `cap`
+    ScoreCap cap;
     float cap_reach;
     float cap_poly[4];
     // kShaped, kCapped
@@ -289,22 +289,23 @@ __device__ __forceinline__ float row_min(const float (&sc)[2][32]) {
 // `rel` is the first key's position relative to the query's.  Returns what is still to be added to each score, the bias of
 // the first key.
 template <bool kCap>
-__device__ __forceinline__ float shape_scores(float (&sc)[2][32], float slope2, int rel, const PrefillParams &p) {
+__device__ __forceinline__ float shape_scores(float (&sc)[2][32], float slope2, int rel, bool row_used, const PrefillParams &p) {
     const float2 c2 = make_float2(p.scale_log2, p.scale_log2), s2 = make_float2(slope2, slope2);
+    auto shape = [&](auto scaled) {
 #pragma unroll
-    for (int cc = 0; cc < 2; ++cc)
+        for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            float2 y = make_float2(sc[cc][i], sc[cc][i + 1]);
-            if (kCap) {
-                y.x = p.cap_log2 - __fdividef(2.f * p.cap_log2, 1.f + fast_exp2(y.x * p.cap_in));
-                y.y = p.cap_log2 - __fdividef(2.f * p.cap_log2, 1.f + fast_exp2(y.y * p.cap_in));
-            } else {
-                y = __fmul2_rn(y, c2);
+            for (int i = 0; i < 32; i += 2) {
+                float2 y = scaled(make_float2(sc[cc][i], sc[cc][i + 1]));
+                y = __ffma2_rn(make_float2(static_cast<float>(cc * 32 + i), static_cast<float>(cc * 32 + i + 1)), s2, y);
+                sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
             }
-            y = __ffma2_rn(make_float2(static_cast<float>(cc * 32 + i), static_cast<float>(cc * 32 + i + 1)), s2, y);
-            sc[cc][i] = y.x, sc[cc][i + 1] = y.y;
-        }
+    };
+    if (!kCap) shape([&](float2 x) { return __fmul2_rn(x, c2); });
+    else if (p.cap.low) shape([&](float2 x) { return make_float2(capped_low(x.x, p.cap), capped_low(x.y, p.cap)); });
+    else if (!__any_sync(0xffffffffu, row_used && fmaxf(row_max(sc), -row_min(sc)) >= p.cap.edge))
+        shape([&](float2 x) { return capped_near(x, p.scale_log2, p.cap); });
+    else shape([&](float2 x) { return capped_any(x, p.scale_log2, p.cap); });
     return slope2 * static_cast<float>(rel);
 }
 // Q of the cap for a pair of squares.
@@ -1108,7 +1109,7 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                     };
                     // a half-step that a row sees nothing of (or scores of -inf): any finite maximum serves
                     auto shaped = [&]() {
-                        const float bias0 = shape_scores<MODE == kCapped>(sc, slope2, key0 - pos, p);      // bias of the first key
+                        const float bias0 = shape_scores<MODE == kCapped>(sc, slope2, key0 - pos, row_used, p);      // bias of the first key
                         mask();
                         if (!new_maximum(fmaxf(row_max(sc) + bias0, -3.0e38f))) return false;
                         const float2 negm2 = make_float2(bias0 - m_run, bias0 - m_run);
@@ -1297,8 +1298,7 @@ inline void fill_geometry(const PrefillCall &c, const PrefillLaunch &l, PrefillP
 inline void fill_shaping(const PrefillCall &c, PrefillParams &p) {
     static const double fit[4] = {0.999997851257, -0.333140392051, 0.130578560594, -0.0409294240958};
     const double per = c.score_cap > 0.f ? (double)c.scale / c.score_cap : 0.0;
-    p.cap_in = static_cast<float>(2.0 * 1.4426950408889634 * per);
-    p.cap_log2 = c.score_cap * 1.4426950408889634f;
+    p.cap = make_score_cap(c.scale, c.score_cap);
     // the coefficients fall by per^2 each: far outside the usual range they would leave fp32's, and no score takes them
     const bool usual = fabs(per) > 1e-4 && fabs(per) < 1e4 && c.score_cap > 1e-6f && c.score_cap < 1e6f;
     p.cap_reach = usual ? static_cast<float>(0.6 / fabs(per)) : 0.f;
