@@ -293,7 +293,9 @@ int npd_paged_scored_prefill_attention(void *out, const void *q, const void *k_c
  * share nothing.  Small batches are answered by one launch without sharing.  num_groups between 1 and 4096, num_q_heads/num_kv_heads <= 128; other shapes
  * as in (2), without the interleaved layouts; `status` and `flags` as in (7).  `workspace`:
  * npd_shared_prefix_workspace_bytes(...) bytes, 256-byte aligned, zeroed once; two calls that may
- * overlap on the GPU need two workspaces.                                                   */
+ * overlap on the GPU need two workspaces.  A call is up to three launches that hand data over in
+ * the workspace: host threads that share a stream and a workspace make their calls one after the
+ * other.                                                                                      */
 size_t npd_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t num_q_heads,
                                          int64_t num_kv_heads, int64_t head_dim, int device);
 int npd_paged_shared_prefix_attention(void *out, const void *q, const void *k_cache,

@@ -68,16 +68,18 @@ def release_workspaces(device=None) -> None:
         keys = [k for k in _workspaces if idx is None or k[0] == idx]
         for d in {k[0] for k in keys}:
             torch.cuda.synchronize(d)
-        scratch_keys = [k for k in _scratch if idx is None or k[0] == idx]
-        for d in {k[0] for k in scratch_keys} - {k[0] for k in keys}:
-            torch.cuda.synchronize(d)
         for k in keys:
             del _workspaces[k]
-        for k in scratch_keys:
-            del _scratch[k]
+    scratch_keys = [k for k in list(_scratch) if idx is None or k[0] == idx]
+    dropped = []
+    for k in scratch_keys + [k for k in list(_captured_scratch) if idx is None or k[0] == idx]:
+        with _scratch_lock(*k):                # no call of another thread is between its scratch and its launches
             _scratch_at.pop(k, None)
-        for k in [k for k in _captured_scratch if idx is None or k[0] == idx]:
-            del _captured_scratch[k]           # the graph's own pool keeps the memory
+            dropped.append(_scratch.pop(k, None))
+            _captured_scratch.pop(k, None)     # the graph's own pool keeps the memory
+    for d in {k[0] for k in scratch_keys}:
+        torch.cuda.synchronize(d)              # before the memory goes back
+    del dropped
 
 
 def check_status(device=None, raise_on_error: bool = True) -> int:
@@ -107,9 +109,11 @@ def check_status(device=None, raise_on_error: bool = True) -> int:
                 bits |= seen
                 word.zero_()
                 if seen & _lib.NPD_STATUS_WAIT_TIMEOUT:
-                    for k, ws in list(_scratch.items()):
-                        if k[0] == idx:
-                            ws.zero_()
+                    for k in [k for k in list(_scratch) if k[0] == idx]:
+                        with _scratch_lock(*k):
+                            if k in _scratch:
+                                _scratch[k].zero_()
+                                torch.cuda.synchronize(idx)
                 torch.cuda.synchronize(idx)
     if bits and raise_on_error:
         names = [n for n, b in (("bad block id", 1), ("bad position / seq_len", 2), ("wait time-out", 4)) if bits & b]
@@ -174,7 +178,12 @@ def _ws_ptr(dev_index: int, handle: int, nbytes: int):
 # stream.  A call that is being captured takes scratch that belongs to its capture (allocated from the graph's own
 # pool, cleared by a node of the graph): two graphs captured on one stream may then be replayed side by side.  The
 # status bits of all of them go to one word per device, which lives as long as the process.
+# Threads may share a stream (all threads of a program begin on the same one): a call holds the stream's lock from the
+# choice of its scratch to its last launch.  A shared-prefix call is three launches that hand plan and rows over in the
+# scratch, another thread's must not come between them; and a call that needs a larger buffer must not give back the
+# one that another call is about to launch on.  One lock per stream: a launch may wait for room in its stream's queue.
 # ---------------------------------------------------------------------------
+_scratch_locks: Dict[Tuple[int, int], "threading.RLock"] = {}
 _scratch: Dict[Tuple[int, int], torch.Tensor] = {}
 _scratch_at: Dict[Tuple[int, int], Tuple[int, int]] = {}            # address and size of each, for the common path
 _packed_call = _C.npd_call_packed
@@ -216,9 +225,15 @@ def _status_ptr(dev_index: int) -> int:
     return address
 
 
+def _scratch_lock(dev_index: int, handle: int):
+    key = (dev_index, handle)
+    lock = _scratch_locks.get(key)
+    return lock if lock is not None else _scratch_locks.setdefault(key, threading.RLock())
+
+
 def _scratch_for(dev_index: int, handle: int, nbytes: int, cleared: int) -> Tuple[int, int]:
     """Address and size of at least ``nbytes`` of scratch for a call on the stream ``handle`` of device ``dev_index``, the first
-    ``cleared`` bytes zero when it is first used."""
+    ``cleared`` bytes zero when it is first used.  The caller holds the stream's lock until it has launched."""
     key = (dev_index, handle)
     capture_id = 0
     if _capturing() or _current_device() != dev_index:          # the first asks about the current device's stream only
@@ -636,11 +651,12 @@ def paged_scored_attention(out, query, key_cache, value_cache, block_tables, seq
         _remember(_scored_plans, key, plan)
     dev_index, need, cleared, flags, cap, win, args = plan
     handle = _raw_stream(dev_index)
-    ws, ws_bytes = _scratch_for(dev_index, handle, need, cleared)
-    _packed_op(_lib.NPD_OP_SCORED_ATTENTION, _pack_scored,
-        dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-        scale, cap, 0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws, ws_bytes,
-        _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
+    with _scratch_lock(dev_index, handle):
+        ws, ws_bytes = _scratch_for(dev_index, handle, need, cleared)
+        _packed_op(_lib.NPD_OP_SCORED_ATTENTION, _pack_scored,
+            dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+            scale, cap, 0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws, ws_bytes,
+            _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
@@ -693,10 +709,11 @@ def paged_shared_prefix_attention(out, query, key_cache, value_cache, block_tabl
         _remember(_shared_plans, key, plan)
     dev_index, need, cleared, flags, args = plan
     handle = _raw_stream(dev_index)
-    ws, ws_bytes = _scratch_for(dev_index, handle, need, cleared)
-    _packed_op(_lib.NPD_OP_SHARED_PREFIX_ATTENTION, _pack_shared,
-        dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-        group_offsets.data_ptr(), shared_lens.data_ptr(), scale, *args, ws, ws_bytes, _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
+    with _scratch_lock(dev_index, handle):
+        ws, ws_bytes = _scratch_for(dev_index, handle, need, cleared)
+        _packed_op(_lib.NPD_OP_SHARED_PREFIX_ATTENTION, _pack_shared,
+            dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+            group_offsets.data_ptr(), shared_lens.data_ptr(), scale, *args, ws, ws_bytes, _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------
@@ -756,12 +773,13 @@ def paged_scored_prefill_attention(out, query, key_cache, value_cache, block_tab
     if nchunks == 0 or total == 0:
         return
     handle = _raw_stream(dev_index)
-    ws, ws_bytes = _scratch_for(dev_index, handle, 256, 256)
-    _packed_op(_lib.NPD_OP_SCORED_PREFILL_ATTENTION, _pack_scored_prefill,
-        dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-        offs.buffer_info()[0], toks.buffer_info()[0], starts.buffer_info()[0], nchunks, scale, cap,
-        0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws, ws_bytes,
-        _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
+    with _scratch_lock(dev_index, handle):
+        ws, ws_bytes = _scratch_for(dev_index, handle, 256, 256)
+        _packed_op(_lib.NPD_OP_SCORED_PREFILL_ATTENTION, _pack_scored_prefill,
+            dev_index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+            offs.buffer_info()[0], toks.buffer_info()[0], starts.buffer_info()[0], nchunks, scale, cap,
+            0 if distance_slopes is None else distance_slopes.data_ptr(), win, *args, ws, ws_bytes,
+            _status_addresses.get(dev_index) or _status_ptr(dev_index), flags, handle)
 
 
 # ---------------------------------------------------------------------------

@@ -3,12 +3,13 @@ launch if the number of CTAs were not limited."""
 import os
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
 import torch
 
-from test_gpu_shared_prefix import check, make
+from test_gpu_shared_prefix import call, check, make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -31,6 +32,34 @@ def test_idle_slots_whose_rows_name_other_pages(kernels, hq, hkv, d, max_ctas, i
     out = check(kernels, (q, kc, vc, bt, sl, go, sh), max_ctas=max_ctas)
     for i in idle:
         assert (out[2 + i] == 0).all()
+
+
+def test_threads_on_one_stream(kernels):
+    """Four threads on the default stream, each with its own batch (of its own size, so that the scratch grows between the
+    calls): three launches a call, none of them another call's."""
+    kernels.release_workspaces()
+    states = [make([(64 * (i + 1), [5 + i, 40, 7]), (512, [3 + j for j in range(4 + 20 * i)])], 12, 2, 128, 16, torch.float16, seed=i) for i in range(4)]
+    outs, errors = [[] for _ in states], []
+
+    def work(i):
+        try:
+            for _ in range(40):
+                out = torch.full_like(states[i][0], float("nan"))
+                call(kernels, out, *states[i], max_ctas=140)
+                outs[i].append(out)
+        except Exception as e:                                  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(states))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for s, got in zip(states, outs):
+        want = check(kernels, s, max_ctas=140)
+        assert all(torch.equal(o, want) for o in got)
 
 
 def test_an_odd_number_of_stages_of_a_cta(kernels):
