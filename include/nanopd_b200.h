@@ -319,7 +319,8 @@ int npd_paged_shared_prefix_attention(void *out, const void *q, const void *k_ca
  * Rows are `hidden` contiguous elements, `*_row_stride` elements apart; gate_row_stride 0 = one
  * gate row for all.  f16 / bf16 / f32, all tensors of one type; hidden a multiple of 8 up to
  * NPD_NORMS_MAX_HIDDEN; pointers and strides multiples of 16 bytes.  residual_out and out may
- * each be x or residual (the same rows at the same stride); no other overlap.               */
+ * each be x or residual (the same rows at the same stride); no other overlap, the weights and the
+ * gate included.                                                                            */
 #define NPD_NORMS_MAX_HIDDEN 32768
 int npd_residual_norms(void *residual_out, void *out, const void *x, const void *residual,
                        const void *weight, const void *post_weight, const void *gate,

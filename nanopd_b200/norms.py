@@ -35,6 +35,12 @@ def _apart(a: int, a_bytes: int, a_stride: int, b: int, b_bytes: int, b_stride: 
     return a_stride == b_stride and row <= (a - b) % a_stride <= a_stride - row
 
 
+def _clear_of(w: int, po: int, eo: int, to: int, ph: int, eh: int, th: int, row: int) -> bool:
+    """Whether the ``row`` bytes of a weight at ``w`` lie beside both outputs: outside their extent or between their rows."""
+    return ((po + eo <= w or w + row <= po or row <= (w - po) % to <= to - row)
+            and (ph + eh <= w or w + row <= ph or row <= (w - ph) % th <= th - row))
+
+
 def residual_norms(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
                    gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0, eps: float = 1e-6, weight_offset: float = 0.0,
                    residual_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
@@ -46,7 +52,7 @@ def residual_norms(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor
 
     ``x``, ``residual``: ``[T, H]`` of one dtype (fp16, bf16, fp32) with contiguous rows, H a multiple of 8 up to 32768; ``weight``,
     ``post_weight``: ``[H]``; ``gate``: ``[H]`` or ``[T, H]``.  ``residual_out`` and ``out`` are allocated when absent; each may be
-    the very rows of ``x`` or of ``residual`` (in place), other overlaps are refused.
+    the very rows of ``x`` or of ``residual`` (in place), other overlaps (with the weights and the gate too) are refused.
     """
     try:
         # one flat key: what the checks look at (the launches are short, and nested tuples cost as much as the checks)
@@ -94,6 +100,7 @@ def residual_norms(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor
     if args[0] == 0:
         return residual_out, out
     px, pr, po, ph, pg = x.data_ptr(), residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(), 0 if gate is None else gate.data_ptr()
+    pw, pp = weight.data_ptr(), 0 if post_weight is None else post_weight.data_ptr()
     if given:
         # a row's values are all read before its outputs are written: an output may be the very rows of x or of the residual
         (ex, tx), (er, tr), (eo, to), (eh, th) = sx, sr, so, sh
@@ -102,8 +109,8 @@ def residual_norms(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor
                 and (ph + eh <= px or px + ex <= ph or (ph == px and th == tx) or _apart(ph, eh, th, px, ex, tx, row))
                 and (ph + eh <= pr or pr + er <= ph or (ph == pr and th == tr) or _apart(ph, eh, th, pr, er, tr, row))
                 and (po + eo <= ph or ph + eh <= po or _apart(po, eo, to, ph, eh, th, row))
-                and (pg == 0 or (_apart(po, eo, to, pg, *sg, row) and _apart(ph, eh, th, pg, *sg, row)))):
+                and (pg == 0 or (_apart(po, eo, to, pg, *sg, row) and _apart(ph, eh, th, pg, *sg, row)))
+                and _clear_of(pw, po, eo, to, ph, eh, th, row) and (pp == 0 or _clear_of(pp, po, eo, to, ph, eh, th, row))):
             raise RuntimeError("residual_norms: an output overlaps another tensor without being the same rows of x or residual")
-    _packed_op(NPD_OP_RESIDUAL_NORMS, _pack, dev_index, po, ph, px, pr, weight.data_ptr(), 0 if post_weight is None else post_weight.data_ptr(),
-               pg, residual_scale, eps, weight_offset, *args, _raw_stream(dev_index))
+    _packed_op(NPD_OP_RESIDUAL_NORMS, _pack, dev_index, po, ph, px, pr, pw, pp, pg, residual_scale, eps, weight_offset, *args, _raw_stream(dev_index))
     return residual_out, out
