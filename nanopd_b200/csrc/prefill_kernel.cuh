@@ -932,7 +932,9 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                 const int U = it.nhalf[x];
                 if (U == 0 || !ok) continue;
                 if (!(ok = wait_or_abort(smem_u32(&ctrl->epi_ready[x]), items_done[x] & 1, abort_flag, p.status))) continue;
-                const float inv = 1.f / ctrl->l_sum[x][row];
+                const float l = ctrl->l_sum[x][row];
+                // a piece of the prefix in which a row has no weight joins as zeros (its log2 sum is -inf)
+                const float inv = MODE == kPrefix && l == 0.f ? 0.f : 1.f / l;
                 // the item's last PV product (products complete in order, so all of them)
                 const int last = c[x] + U - 1;
                 if (!(ok = wait_or_abort(smem_u32(&ctrl->pv_done[x][last & 1]), (last >> 1) & 1, abort_flag, p.status))) continue;
@@ -1150,7 +1152,9 @@ paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap 
                             for (int i = 0; i < 32; ++i)
                                 if (key0 + cc * 32 + i > pos) sc[cc][i] = -INFINITY;
                     }
-                    if (!(ok = new_maximum(row_max(sc) * p.scale_log2))) break;
+                    float m_new = row_max(sc) * p.scale_log2;
+                    if (MODE == kPrefix) m_new = fmaxf(m_new, -3.0e38f);      // scores that are all -inf: any finite maximum serves
+                    if (!(ok = new_maximum(m_new))) break;
                     if (lane == 0) NPD_TRACE_FINE(sm_role, 23, u);
                     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), negm2 = make_float2(-m_run, -m_run);
                     probabilities([&](float2 y) { return __ffma2_rn(y, scale2, negm2); });

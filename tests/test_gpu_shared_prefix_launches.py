@@ -34,6 +34,21 @@ def test_idle_slots_whose_rows_name_other_pages(kernels, hq, hkv, d, max_ctas, i
         assert (out[2 + i] == 0).all()
 
 
+@pytest.mark.parametrize("max_ctas", [0, 140, 2])
+def test_keys_whose_scores_are_minus_infinity(kernels, max_ctas):
+    """Pages of the prefix, whole pieces of it and all own tokens of a sequence may score -inf: they weigh nothing, and the rest
+    of the row is what it is without them."""
+    q, kc, vc, bt, sl, go, sh = make([(640, [5, 20, 100, 33]), (256, [3, 40])], 12, 2, 128, 16, torch.float16)
+    q.fill_(1.0)
+    kc[bt[0, :9].long(), :, :, 3] = float("-inf")               # more than the first key tile of the first group
+    kc[bt[0, 20:37].long(), :, :, 3] = float("-inf")
+    kc[bt[4, 8:16].long(), :, :, 7] = float("-inf")             # the whole second tile of the second
+    kc[bt[1, 40:42].long(), :, :, 9] = float("-inf")            # every own token of sequence 1
+    check(kernels, (q, kc, vc, bt, sl, go, sh), max_ctas=max_ctas)
+    kc[bt[4, :16].long(), :, :, 7] = float("-inf")              # the whole prefix of the second group
+    check(kernels, (q, kc, vc, bt, sl, go, sh), max_ctas=max_ctas)
+
+
 def test_threads_on_one_stream(kernels):
     """Four threads on the default stream, each with its own batch (of its own size, so that the scratch grows between the
     calls): three launches a call, none of them another call's."""
