@@ -44,6 +44,7 @@ class StepContext:
     # host-side work estimates behind the SM split of a mixed step
     prefill_score_pairs: int = 0                       # sum over prompt chunks of n*start + n(n+1)/2
     decode_context_tokens: int = 0                     # sum over decode sequences of position + 1
+    decode_lens: Optional[np.ndarray] = None           # position + 1 of each, for steps with a window
 
 
 def _padded_table(rows: List[List[int]]) -> np.ndarray:
@@ -95,7 +96,8 @@ def build_step_context(ctx: Dict, device, block_size: int = 16) -> StepContext:
                 raise RuntimeError("a decode position lies beyond its block table")
         parts["decode_positions"] = positions
         parts["decode_seq_lens"] = positions + 1
-        sc.decode_context_tokens = int(positions.sum()) + len(decodes)
+        sc.decode_lens = positions.astype(np.int64) + 1
+        sc.decode_context_tokens = int(sc.decode_lens.sum())
 
     # one staging buffer, 256-byte aligned sections, one copy
     offsets, total = {}, 0
@@ -124,19 +126,36 @@ def build_step_context(ctx: Dict, device, block_size: int = 16) -> StepContext:
 # one CTA per SM.  Run one after the other, each leaves the other's resource idle.  In a mixed step they are
 # launched side by side instead, each capped to its share of the SMs; the split minimises the longer of the two
 # estimated times.
-_PREFILL_FLOPS_PER_S = 1.1e15      # measured rates of the two kernels on a B200, only used for the split
+# measured rates of the two kernels on a B200, only used for the split.  Prompts: by how many of cap and distance bias a score
+# takes (512-token chunks of four prompts in graph replays, TFLOP/s: a cap 945, a bias 900, both 510; 4096-token windows
+# alone run at the plain kernel's rate)
+_PREFILL_FLOPS_PER_S = (1.1e15, 0.9e15, 0.5e15)
 _DECODE_BYTES_PER_S = 6.0e12
 _MIN_OVERLAP_SECONDS = 15e-6       # below this much estimated work on either side, fork and join cost more than they save
 _side_streams: Dict[int, "torch.cuda.Stream"] = {}
 
 
-def _sm_split(sc: StepContext, hq: int, hkv: int, d: int, elem: int, sms: int) -> Optional[int]:
+def _visible_work(sc: StepContext, window: int) -> tuple:
+    """(score pairs of the prompt chunks, tokens that the decode sequences read) under a window, 0 = none."""
+    if window <= 0:
+        return sc.prefill_score_pairs, sc.decode_context_tokens
+    pairs = 0
+    for n, start in zip(sc.prefill_tokens, sc.prefill_starts):
+        short = min(n, max(0, window - start))                  # queries that still see everything before them
+        pairs += short * start + short * (short + 1) // 2 + (n - short) * window
+    if sc.decode_lens is None:
+        return pairs, min(sc.decode_context_tokens, sc.num_decode_tokens * window)
+    return pairs, int(np.minimum(sc.decode_lens, window).sum())
+
+
+def _sm_split(sc: StepContext, hq: int, hkv: int, d: int, elem: int, sms: int, window: int = 0, shapings: int = 0) -> Optional[int]:
     """Of ``sms`` SMs, how many the prompt chunks get in a mixed step (the rest go to the decode batch);
-    None = run the two kernels in turn."""
+    None = run the two kernels in turn.  ``shapings``: how many of cap and distance bias the scores take."""
     if sc.num_prefill_tokens == 0 or sc.num_decode_tokens == 0 or sms < 64:
         return None
-    t_p = 4.0 * hq * d * sc.prefill_score_pairs / _PREFILL_FLOPS_PER_S
-    t_d = 2.0 * hkv * d * elem * sc.decode_context_tokens / _DECODE_BYTES_PER_S
+    pairs, tokens = _visible_work(sc, window)
+    t_p = 4.0 * hq * d * pairs / _PREFILL_FLOPS_PER_S[shapings]
+    t_d = 2.0 * hkv * d * elem * tokens / _DECODE_BYTES_PER_S
     if min(t_p, t_d) < _MIN_OVERLAP_SECONDS:
         return None
     # The decode kernel switches to 12 warps per CTA on a capped grid and then keeps HBM saturated down to about
@@ -164,7 +183,8 @@ def _attend(sc: StepContext, out, q_tokens_major, k_cache, v_cache, scale, overl
     _, hq, d = q_tokens_major.shape
     dev = q_tokens_major.device
     sms = torch.cuda.get_device_properties(dev).multi_processor_count
-    share = _sm_split(sc, hq, k_cache.size(1), d, q_tokens_major.element_size(), sms) if overlap else None
+    share = _sm_split(sc, hq, k_cache.size(1), d, q_tokens_major.element_size(), sms, window,
+                      (score_cap != 0) + (distance_slopes is not None)) if overlap else None
 
     def prefill(max_ctas=0):
         prefill_op(out[:P], q_tokens_major[:P], k_cache, v_cache, sc.prefill_tables, sc.prefill_offsets, sc.prefill_tokens,
