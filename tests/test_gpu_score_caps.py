@@ -31,12 +31,10 @@ def test_large_caps_in_prompts(kernels, hq, hkv, d, cap):
     prompt.check(kernels, q, kc, vc, bt, chunks, cap, prompt.slopes_for(hq), 90)
 
 
-@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("cap", [c for c in CAPS if c >= 1e5])
 def test_a_large_cap_changes_nothing_that_the_scores_show(kernels, cap):
     """A cap a thousand times the largest score and more moves a score by less than 1e-6 of it; the plain form of the same
     operator is that close.  (Probabilities move by 2^-11 or less in fp16, and by 15 * 1.2e-6 through the score.)"""
-    if cap < 1e5:
-        pytest.skip("the cap is to be far above the scores")
     chunks = [(0, 250)]
     q, kc, vc, bt = prompt.make(chunks, 12, 2, 128, 16, torch.float16, gain=3.0)
     out, plain = torch.empty_like(q), torch.empty_like(q)

@@ -9,10 +9,51 @@ from pathlib import Path
 import pytest
 import torch
 
+import test_gpu_shared_prefix as one_launch
+from nanopd_b200 import paged_kernels
 from test_gpu_shared_prefix import call, check, make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+@pytest.fixture()
+def limited(kernels):
+    """The operators with the number of CTAs limited, which switches the one-launch form off."""
+    class Limited:
+        @staticmethod
+        def paged_shared_prefix_attention(*args, **kw):
+            kernels.paged_shared_prefix_attention(*args, **{"max_ctas": 140, **kw})
+
+        def __getattr__(self, name):
+            return getattr(kernels, name)
+
+    return Limited()
+
+
+@pytest.mark.parametrize("shared", [0, 15, 16, 17, 31, 32, 63, 64, 65, 127, 128, 129, 255, 1000, 4112])
+def test_lengths_of_the_prefix(limited, shared):
+    one_launch.test_lengths_of_the_prefix(limited, shared)
+
+
+@pytest.mark.parametrize("case", ["test_prefix_that_is_the_whole_of_some_sequences", "test_idle_slots_in_a_group", "test_large_scores",
+                                  "test_groups_that_do_not_ascend_share_nothing", "test_agrees_with_the_plain_operator_and_repeats_bit_for_bit",
+                                  "test_rows_behind_the_batch_and_strided_tables", "test_graphs_with_changing_lengths_and_side_streams",
+                                  "test_many_sequences_and_many_groups"])
+def test_cases_of_the_one_launch_form(limited, case):
+    """Prefixes that the shortest sequence cuts, offsets that do not ascend, replays of one graph with other lengths, graphs
+    replayed side by side: through plan, prefix pass and tail."""
+    getattr(one_launch, case)(limited)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(32, 1, 128), (16, 16, 64), (16, 2, 256)])
+@pytest.mark.parametrize("max_ctas", [1, 2, 9])
+def test_hundreds_of_short_pieces_to_a_cta(kernels, hq, hkv, d, max_ctas):
+    """Prefixes of one key tile and groups of two: items that give the second query tile no work follow one another."""
+    state = make([(16 * (1 + i % 4), [1 + (i + j) % 9 for j in range(2)]) for i in range(150)], hq, hkv, d, 16, torch.bfloat16)
+    first = check(kernels, state, max_ctas=max_ctas)
+    for _ in range(5):
+        assert torch.equal(check(kernels, state, max_ctas=max_ctas), first)
 
 
 @pytest.mark.parametrize("idle", [(0,), (0, 1), (2,), (0, 3), (1, 2, 3)])
@@ -52,7 +93,7 @@ def test_keys_whose_scores_are_minus_infinity(kernels, max_ctas):
 def test_threads_on_one_stream(kernels):
     """Four threads on the default stream, each with its own batch (of its own size, so that the scratch grows between the
     calls): three launches a call, none of them another call's."""
-    kernels.release_workspaces()
+    paged_kernels.release_workspaces()
     states = [make([(64 * (i + 1), [5 + i, 40, 7]), (512, [3 + j for j in range(4 + 20 * i)])], 12, 2, 128, 16, torch.float16, seed=i) for i in range(4)]
     outs, errors = [[] for _ in states], []
 
