@@ -247,7 +247,8 @@ int npd_top_k_sample(int64_t *out_ids, const void *logits, const float *uniforms
  * may name pages that belong to someone else by now.  What the page slots before the window and
  * behind the sequence hold (NaN included) does not reach the result.  A sequence with
  * seq_lens[s] == 0 gets a zero row.  Shapes and layouts as in npd_paged_decode_attention, the
- * interleaved layouts excepted; `flags` takes NPD_FLAG_MAX_CTAS.  score_cap must be 0
+ * interleaved layouts excepted; `flags` takes NPD_FLAG_MAX_CTAS.  seq_lens may change between
+ * launches, not while one runs (the rows and the workspace are then undefined).  score_cap must be 0
  * or between 1e-30 and 1e38, window not negative, scale finite and not negative (in (8) and (9) too).  `workspace`: npd_decode_workspace_bytes(...) bytes,
  * zeroed once, as there; a launch leaves its tickets at zero.  `status` (device int32, may be
  * NULL) receives the NPD_STATUS_* bits; when NULL the workspace's first word does.          */

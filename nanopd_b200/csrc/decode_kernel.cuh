@@ -851,7 +851,7 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
                 my_id = checked(table_lookup(win, pc.s, tok0 >> p.block_shift, npages, lane, p));
             } else {
                 // several boxes to a tile; those wholly before the window or behind the sequence are not read
-                boxes = min(kTile, pc.len - tok0 + p.box_rows - 1) >> p.box_shift;
+                boxes = max(0, min(kTile, pc.len - tok0 + p.box_rows - 1)) >> p.box_shift;
                 if (MODE == kScored) first_box = max(0, first_visible<MODE>(p, pc.len) - tok0) >> p.box_shift;
                 for (int k = first_box; k < boxes; ++k) {
                     const int id = checked(table_lookup(win, pc.s, (tok0 + (k << p.box_shift)) >> p.block_shift, npages, lane, p));
@@ -968,7 +968,8 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
             uint8_t *vt = kt + TILE_BYTES;
             const uint32_t ks_addr = smem_u32(kt), vs_addr = smem_u32(vt);
             const int tok0 = (seg_first + t_first + it) * kTile;
-            const int valid = min(kTile, seg_len - tok0);
+            // (lengths are read more than once: should they change under the kernel, no row outside the tile is touched)
+            const int valid = max(0, min(kTile, seg_len - tok0));
 
             if (valid < kTile) {
                 // V rows past the sequence end may hold anything (NaN included): P is exactly 0
@@ -993,7 +994,7 @@ paged_decode_stream_kernel(const DecodeParams p, const __grid_constant__ CUtenso
             const int seg_lo = first_visible<MODE>(p, seg_len);
             if (MODE == kScored && tok0 < seg_lo) {
                 // likewise the V rows before the window
-                const int cnt = (seg_lo - tok0) * NH * 8;
+                const int cnt = min(seg_lo - tok0, kTile) * NH * 8;
                 for (int idx = lane; idx < cnt; idx += 32) {
                     const int r = idx / (NH * 8), c = idx % (NH * 8);
                     *reinterpret_cast<uint4 *>(vt + tile_offset<D>(r, c, p.box_rows)) = make_uint4(0, 0, 0, 0);
