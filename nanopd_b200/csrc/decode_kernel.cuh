@@ -85,7 +85,6 @@ struct DecodeParams {
     const PrefixPlanHead *plan_head;
     const float *prefix_o;        // [rows][D] normalised rows of the pieces
     const float *prefix_lse;      // [rows] log2 of the pieces' softmax sums, maximum included
-    int num_kv_heads;             // physical
     int group_full;               // q heads per physical kv head
 };
 
@@ -1255,16 +1254,19 @@ void consider_small_form(LaunchShape &ls, int head_dim, long long max_tokens, lo
     while (ls.nstages > 1 && (long long)ls.nwarps * ls.nstages * stage_bytes > 192 * 1024) --ls.nstages;
 }
 
-// kScored's small form: a cluster of CTAs to a (sequence, kv head), as many as leave every cluster a place (clusters of 8 of
-// these CTAs, one to an SM, fit 16 at a time), up to kClusterTokens tokens per CTA; beyond that the streaming form's equal
-// split wins.  Device time per launch, small form / streaming form (32/8 heads of 128, capped): 1 sequence of 256 tokens
-// 7.2 / 11.2 us, of 2048 10 / 19, of 8192 17.5 / 32, of 16000 32 / 43; 8 of 2000 18.6 / 27; 16 of 1000 17.6 / 24.6; 70 of 1000
-// (12/2 heads) 18.3 / 26.  Twelve warps to a CTA: 8 of 2000 20.4 us with eight.
+// kScored's small form: a cluster of CTAs to a (sequence, kv head), as many as leave every cluster a place, up to kClusterTokens
+// tokens per CTA; beyond that the streaming form's equal split wins.  Of clusters of eight (one CTA to an SM, all of them in one
+// GPC) 15 fit at a time on a B200, so sixteen pairs take clusters of four as far as those reach: 2000 / 8000 tokens of head size
+// 128 9.5 / 19.2 us against 15.9 / 25.8 in two turns of clusters of eight; beyond it the two turns still win (12000 tokens 31
+// against 35 us streaming).  Device time per launch, small form / streaming form (32/8 heads of 128, capped): 1 sequence of
+// 256 tokens 7.2 / 11.2 us, of 2048 10 / 19, of 8192 17.5 / 32, of 16000 32 / 43; 8 of 2000 18.6 / 27; 16 of 1000 17.6 / 24.6;
+// 70 of 1000 (12/2 heads) 18.3 / 26.  Twelve warps to a CTA: 8 of 2000 20.4 us with eight.
 constexpr long long kClusterTokens = 2176;
 constexpr int kClusterWarps = 12;
 void consider_cluster_form(LaunchShape &ls, int head_dim, long long max_tokens, long long seq_heads, int cta_cap, int flags, int device) {
     if ((flags & NPD_DECODE_NO_SMALL) || cta_cap > 0 || seq_heads < 1 || seq_heads > npd::sm_count(device)) return;
-    int cluster = seq_heads <= 16 ? 8 : (seq_heads <= 32 ? 4 : (seq_heads <= 64 ? 2 : 1));
+    int cluster = seq_heads <= 15 ? 8 : (seq_heads <= 32 ? 4 : (seq_heads <= 64 ? 2 : 1));
+    if (seq_heads == 16 && max_tokens > kClusterTokens * cluster) cluster = 8;
     if (max_tokens > kClusterTokens * cluster) return;
     const int nwarps = head_dim == 256 ? 8 : kClusterWarps;
     // a warp has a tile at least
@@ -1566,7 +1568,6 @@ int run_decode(const DecodeCall &c) {
     p.plan_head = c.plan_head;
     p.prefix_o = c.prefix_o;
     p.prefix_lse = c.prefix_lse;
-    p.num_kv_heads = static_cast<int>(c.num_kv_heads);
     p.group_full = static_cast<int>(c.num_q_heads / c.num_kv_heads);
 
     const size_t elem = 2;

@@ -6,10 +6,10 @@
 // Three launches on one stream, everything decided on the device (lengths may change between replays of a graph):
 //   plan    one CTA: per group the tokens that all its sequences share and none ends in, in 16-token tiles; the line of
 //           (group, query tiles, kv head, key tile) units cut into equal runs, one per SM; per sequence where its rows are
-//   prefix  prefix_pass.cu: the rows of a group (sequences x heads of a kv head, 256 at a time) over the shared pages on the
-//           tensor cores, a piece per cut, normalised fp32 rows and their log2 sums
+//   prefix  prefix_pass.cu: the rows of a group (sequences x heads of a kv head, 256 at a time, 128 at head size 256) over the
+//           shared pages on the tensor cores, a piece per cut, normalised fp32 rows and their log2 sums
 //   tail    the streaming decode kernel over each sequence's own pages, which joins the pieces where it writes the row
-// Bytes: prefix pages once per 256 rows of a kv head + own pages; flops of the prefix 4 * Hq * D * tokens * sequences.
+// Bytes: prefix pages once per 256 (128) rows of a kv head + own pages; flops of the prefix 4 * Hq * D * tokens * sequences.
 #include "decode_kernel.cuh"
 
 namespace {
@@ -225,8 +225,10 @@ extern "C" int npd_paged_shared_prefix_attention(void *out, const void *q, const
     if (status == nullptr) status = reinterpret_cast<int32_t *>(ws);
     {
         // A small batch whose sequences fit a cluster of CTAs each is answered by that one launch: reading the shared pages
-        // again (they are in L2) costs less than three launches.  16 sequences behind 992 shared tokens, 12/2 heads:
-        // 9.6 us, with sharing 29 us.
+        // again (they are in L2) costs less than three launches.  Measured at 2 to 74 sequences behind 512 to 16000 shared
+        // tokens, 100 of their own, 12/2, 32/8 and 16/16 heads and 16/2 of 256: one launch / sharing 7 / 22 us for 16
+        // sequences (12/2) behind 512 tokens, 8.8 / 24 behind 992, 18 / 25 for 18 sequences (32/8) behind 2000, 35 / 62 for
+        // 37 (16/2 of 256) behind 2000; the one point of 89 where sharing won was 2 sequences (32/8) behind 16000, 36 / 32.
         const npd::SharedCall sc{out, q, k_cache, v_cache, block_tables, seq_lens, group_offsets, shared_lens, scale, num_seqs, num_groups,
                                  num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks, cache_block_stride,
                                  bt_row_stride, dtype, workspace, decode_bytes, status, flags, stream};
