@@ -20,7 +20,8 @@
 //                    which ONE warp can issue tiled copies (about 100 clocks per 2 KiB box) is what bounded the
 //                    kernel when a single warp issued the 32 boxes of a 128-key step
 //   warps 9 / 10     issue the tcgen05.mma instructions of tile A / B (one elected lane) and request the tile's
-//                    query rows (the next item's as soon as this item's last score MMA has completed)
+//                    query rows (the next item's as soon as this item's last score MMA has completed); they clear the V
+//                    rows that nobody may see
 //   warps 12-15      epilogue of both tiles: O / l -> out, while the softmax groups are already on the next item
 // TMEM (512 columns): S_A | S_B | O_A | O_B, 128 columns each.  A query tile walks its keys in HALF-STEPS of 64
 // keys; its 128 score columns are a ring of two 64-column buffers, so the scores of half-step c+1 are
@@ -1296,7 +1297,7 @@ inline void fill_geometry(const PrefillCall &c, const PrefillLaunch &l, PrefillP
 // The cap as a polynomial: tanh(z) = z P(z^2) for |z| < 0.6, P of degree 3 fitted by Remez exchange for the least relative
 // error, 2.1e-6 (at the largest score it serves, cap * tanh(0.6), that is 1.1e-6 cap).  With x = q . k and z = x scale / cap,
 // cap log2(e) tanh(z) = x Q(x^2).  Four multiply-adds a score; an exponential and a reciprocal beside the softmax's own
-// exponential, as for the scores beyond, would bound the kernel by its special-function unit: 16384 scores of a half-step of
+// exponential, as where a score lies beyond, would bound the kernel by its special-function unit: 16384 scores of a half-step of
 // both query tiles at 16 a clock are 1024 clocks for each, the tensor cores need 1024 for the products.  Scores beyond 0.6
 // cap are what a cap is there for, but they are rare.
 inline void fill_shaping(const PrefillCall &c, PrefillParams &p) {

@@ -2,8 +2,7 @@
 // window.  For the query of sequence s (at position n - 1, n = seq_lens[s]) and key j, with n - window <= j < n:
 //   x_j = scale * q . k_j;   x_j = cap * tanh(x_j / cap);   x_j -= slope[h] * (n - 1 - j);   out = softmax(x) . V
 // The kernel is the streaming one of decode_kernel.cuh in its mode kScored: HBM-bound, every visible K/V byte read once.
-// A tile of 16 keys costs a thread four scores, so the tanh (one exponential and one reciprocal) disappears behind the
-// tile's loads.  A window moves the first tile of each sequence: the split into equal work, the small-batch form and the
+// A tile of 16 keys costs a thread four scores, so the tanh (capped_scores.cuh) disappears behind the tile's loads.  A window moves the first tile of each sequence: the split into equal work, the small-batch form and the
 // merge then count its tiles only, and neither the pages before it nor their table entries are read.
 #include "decode_kernel.cuh"
 
